@@ -1,0 +1,487 @@
+// Microscaled (MX) quantisation, its read-back, its straight-through form for calibration, and the root-mean-square norm with the
+// residual's addition that writes its output microscaled.  Every kernel reads each input once and writes each output once; all are
+// bound by memory.
+//
+// Format: a row is cut into blocks of 32 elements; a block holds 32 codes and one byte b, the scale 2^(b - 127):
+//   b - 127 = floor(log2 max|x|) - emax,  emax = 2 (e2m1) / 8 (e4m3);   code = nearest-even element of x 2^-(b - 127), saturating.
+// A row whose length is no multiple of 32 ends in a block filled up with zero codes.
+#include "mx_common.h"
+#include "../../include/edadm.h"
+
+enum { MX_QUANT = 0, MX_FAKE = 1, MX_GRAD = 2 };
+
+// ------------------------------------------------------------------------------------------------ element-wise forms
+// An item is 8 elements of a row; a row has `items` = 4 x blocks of them.  Dense tensors with whole blocks come as ONE row (the
+// host folds them), so the row index is only divided out for ragged or strided rows.  U items per thread, a block's width apart,
+// all loads issued before the first use.
+template <int DT, int FMT, int OP, bool VEC, int U>
+__global__ __launch_bounds__(256) void k_mx_elem(const void* __restrict__ x, int64_t ldx, const void* __restrict__ gy, int64_t ldg,
+                                                 void* __restrict__ out, int64_t ldo, uint8_t* __restrict__ codes, int64_t ldc,
+                                                 uint8_t* __restrict__ scales, int64_t lds, int64_t rows, int64_t cols, int64_t items) {
+    const int64_t total = rows * items, first = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+    float v[U][8], g[U][8];
+    int64_t row[U], it[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = first + u * 256;
+        if (rows == 1) { row[u] = 0; it[u] = i; }
+        else if (total <= 0x7fffffff) { row[u] = (uint32_t)i / (uint32_t)items; it[u] = (uint32_t)i - (uint32_t)row[u] * (uint32_t)items; }
+        else { row[u] = i / items; it[u] = i - row[u] * items; }
+        const int64_t left = cols - it[u] * 8;
+        const int valid = i < total ? (int)(left < 8 ? left : 8) : 0;
+        if (valid > 0) {
+            mx_load8<DT, VEC>(x, row[u] * ldx + it[u] * 8, valid, v[u]);
+            if constexpr (OP == MX_GRAD) mx_load8<DT, VEC>(gy, row[u] * ldg + it[u] * 8, valid, g[u]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { v[u][e] = 0.f; if constexpr (OP == MX_GRAD) g[u][e] = 0.f; }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + u * 256 >= total) break;                          // whole quads: items is a multiple of 4
+        const int64_t left = cols - it[u] * 8;
+        const int valid = (int)(left < 8 ? left : 8);
+        if constexpr (OP == MX_QUANT) {
+            const uint32_t b = mx_block_exp<FMT>(v[u]);
+            mx_put<FMT>(codes + row[u] * ldc, scales + row[u] * lds, it[u], mx_encode8<FMT>(v[u], b, mx_scale(b)), b);
+        } else if constexpr (OP == MX_FAKE) {
+            mx_fake8<FMT>(v[u]);
+            if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, v[u]);
+        } else {
+            const float top = mx_top<FMT>(v[u]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[u][e] = fabsf(v[u][e]) <= top ? g[u][e] : 0.f;
+            if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, g[u]);
+        }
+    }
+}
+
+template <int DT, int FMT, bool VEC, int U>
+__global__ __launch_bounds__(256) void k_mx_read(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
+                                                 int64_t lds, void* __restrict__ out, int64_t ldo, int64_t rows, int64_t cols,
+                                                 int64_t items) {
+    const int64_t total = rows * items, first = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+    uint2 c[U];
+    uint32_t b[U];
+    int64_t row[U], it[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = first + u * 256;
+        if (rows == 1) { row[u] = 0; it[u] = i; }
+        else if (total <= 0x7fffffff) { row[u] = (uint32_t)i / (uint32_t)items; it[u] = (uint32_t)i - (uint32_t)row[u] * (uint32_t)items; }
+        else { row[u] = i / items; it[u] = i - row[u] * items; }
+        c[u] = make_uint2(0, 0);
+        b[u] = 0;
+        if (i < total) {
+            if constexpr (FMT == MX_FP4) c[u].x = *(const uint32_t*)(codes + row[u] * ldc + it[u] * 4);
+            else c[u] = *(const uint2*)(codes + row[u] * ldc + it[u] * 8);
+            b[u] = scales[row[u] * lds + (it[u] >> 2)];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + u * 256 >= total) break;
+        const int64_t left = cols - it[u] * 8;
+        const int valid = (int)(left < 8 ? left : 8);
+        float v[8];
+        mx_decode8<FMT>(c[u], mx_scale(b[u]), v);
+        if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ root-mean-square norm
+// h = x (+ r, rounded to the stream's type);  rstd = 1 / sqrt(mean h^2 + eps);  y = (h rstd) w, each product rounded to 32 bits;
+// the output is y, its quantised form or what that stands for.
+// The mean of squares is summed in 64 bits (two instructions more per element of a kernel bound by memory) and rounded once, so
+// that rstd does not depend on the order of the sum: codes next to a rounding border go by its last bit.
+// A row is held in registers by `tpr` threads, VPT eights each; tpr = 64: four rows to a workgroup, no barrier; else one row.
+enum { RN_PLAIN = 0, RN_FP4 = MX_FP4, RN_FP8 = MX_FP8, RN_FAKE4 = 16 + MX_FP4, RN_FAKE8 = 16 + MX_FP8 };
+
+__device__ __forceinline__ double row_sum(double s, int tpr, double* sm) {
+    s = wave_sum_d(s);
+    if (tpr == 64) return s;
+    const int w = threadIdx.x >> 6, n = tpr >> 6;
+    if ((threadIdx.x & 63) == 0) sm[w] = s;
+    __syncthreads();
+    double t = 0;
+    for (int i = 0; i < n; ++i) t += sm[i];
+    return t;
+}
+
+template <int DT, bool WF32, int VPT, bool VEC>
+__global__ __launch_bounds__(1024) void k_rmsnorm(const void* __restrict__ x, int64_t ldx, const void* __restrict__ r, int64_t ldr,
+                                                  const void* __restrict__ w, void* __restrict__ h, int64_t ldh,
+                                                  float* __restrict__ rstd, void* __restrict__ out, int64_t ldo,
+                                                  uint8_t* __restrict__ scales, int64_t lds, int64_t rows, int64_t cols, int items,
+                                                  double eps, int mode, int tpr) {
+    __shared__ double sm[16];
+    const int t = threadIdx.x % tpr;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+    if (row >= rows) return;                                          // whole waves: tpr is a multiple of 64
+    constexpr int WDT = WF32 ? MX_F32 : DT;
+    float v[VPT][8];
+    double ss = 0;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int it = t + k * tpr;
+        const int64_t left = cols - (int64_t)it * 8;
+        const int valid = (int)(left < 8 ? left : 8);
+        if (valid > 0) {
+            mx_load8<DT, VEC>(x, row * ldx + it * 8, valid, v[k]);
+            if (r) {
+                float q[8];
+                mx_load8<DT, VEC>(r, row * ldr + it * 8, valid, q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] += q[e];
+                mx_round8<DT>(v[k]);
+                mx_store8<DT, VEC>(h, row * ldh + it * 8, valid, v[k]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fma((double)v[k][e], (double)v[k][e], ss);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+        }
+    }
+    ss = row_sum(ss, tpr, sm);
+    const float rs = (float)(1.0 / sqrt(ss / (double)cols + eps));
+    if (rstd && t == 0) rstd[row] = rs;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int it = t + k * tpr;
+        if (it >= items) break;                                       // whole quads
+        const int64_t left = cols - (int64_t)it * 8;
+        const int valid = (int)(left < 8 ? left : 8);
+        float q[8];
+        if (valid > 0) mx_load8<WDT, VEC>(w, (int64_t)it * 8, valid, q);
+        else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[e] = 0.f;
+        }
+        // beyond the row's end the product is kept at 0, whatever rstd is
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[k][e] = VEC ? (valid > 0 ? (v[k][e] * rs) * q[e] : 0.f) : (e < valid ? (v[k][e] * rs) * q[e] : 0.f);
+        if (mode == RN_FP8) {
+            const uint32_t b = mx_block_exp<MX_FP8>(v[k]);
+            mx_put<MX_FP8>((uint8_t*)out + row * ldo, scales + row * lds, it, mx_encode8<MX_FP8>(v[k], b, mx_scale(b)), b);
+        } else if (mode == RN_FP4) {
+            const uint32_t b = mx_block_exp<MX_FP4>(v[k]);
+            mx_put<MX_FP4>((uint8_t*)out + row * ldo, scales + row * lds, it, mx_encode8<MX_FP4>(v[k], b, mx_scale(b)), b);
+        } else {
+            if (mode == RN_FAKE8) mx_fake8<MX_FP8>(v[k]);
+            else if (mode == RN_FAKE4) mx_fake8<MX_FP4>(v[k]);
+            if (valid > 0) mx_store8<DT, VEC>(out, row * ldo + it * 8, valid, v[k]);
+        }
+    }
+}
+
+// Backward.  With g the output's gradient where the element was inside its block's range (0 elsewhere), xh = h rstd:
+//   dh = gh + rstd (g w - xh mean(g w xh)),   dw = sum over rows g xh.
+// The range is found again from h, rstd and w (no mask is kept).  Rows of up to two eights a thread keep w and gh in registers too;
+// four eights would not fit beside them, and read those where they are used.  A workgroup walks rows blockIdx, blockIdx + grid, ...; its share of
+// dw stays in registers and goes out once, as a row of `part`, which k_colsum adds up in a fixed order in 64 bits.
+template <int DT, bool WF32, int VPT, bool VEC>
+__global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ gy, int64_t ldg, const void* __restrict__ gh,
+                                                      int64_t ldgh, const void* __restrict__ h, int64_t ldh,
+                                                      const float* __restrict__ rstd, const void* __restrict__ w,
+                                                      void* __restrict__ dh, int64_t ldd, float* __restrict__ part, int64_t rows,
+                                                      int64_t cols, int items, int fmt, int tpr) {
+    __shared__ double sm[2][16];
+    const int t = threadIdx.x % tpr, slots = blockDim.x / tpr, slot = threadIdx.x / tpr;
+    constexpr int WDT = WF32 ? MX_F32 : DT;
+    constexpr bool HOLD = VPT <= 2;
+    float wh[HOLD ? VPT : 1][8], acc[VPT][8];
+    auto load_w = [&](int k, float (&wv)[8]) {
+        const int64_t left = cols - (int64_t)(t + k * tpr) * 8;
+        const int valid = (int)(left < 8 ? left : 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) wv[e] = 0.f;
+        if (valid > 0) mx_load8<WDT, VEC>(w, (int64_t)(t + k * tpr) * 8, valid, wv);
+    };
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[k][e] = 0.f;
+        if constexpr (HOLD) load_w(k, wh[k]);
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * slots + slot; row < rows; row += (int64_t)gridDim.x * slots, turn ^= 1) {
+        const float rs = rstd[row];
+        float g[VPT][8], xh[VPT][8], uh[HOLD ? VPT : 1][8];
+        double dot = 0;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int it = t + k * tpr;
+            const int64_t left = cols - (int64_t)it * 8;
+            const int valid = (int)(left < 8 ? left : 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { g[k][e] = 0.f; xh[k][e] = 0.f; if constexpr (HOLD) uh[k][e] = 0.f; }
+            if (valid > 0) {
+                mx_load8<DT, VEC>(h, row * ldh + it * 8, valid, xh[k]);
+                mx_load8<DT, VEC>(gy, row * ldg + it * 8, valid, g[k]);
+                if constexpr (HOLD) if (gh) mx_load8<DT, VEC>(gh, row * ldgh + it * 8, valid, uh[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int it = t + k * tpr;
+            if (it >= items) break;                                   // whole quads
+            const int64_t left = cols - (int64_t)it * 8;
+            float y[8], wv[8];
+            if constexpr (HOLD) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) wv[e] = wh[k][e];
+            } else load_w(k, wv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                xh[k][e] *= rs;
+                y[e] = e < left ? xh[k][e] * wv[e] : 0.f;          // the forward's rounding
+            }
+            if (fmt) {
+                const float top = fmt == MX_FP4 ? mx_top<MX_FP4>(y) : mx_top<MX_FP8>(y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[k][e] = fabsf(y[e]) <= top ? g[k][e] : 0.f;
+            }
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                acc[k][e] = fmaf(e < left ? g[k][e] : 0.f, xh[k][e], acc[k][e]);
+                g[k][e] *= wv[e];
+                s = fmaf(g[k][e], xh[k][e], s);
+            }
+            dot += s;
+        }
+        // the two slots of sm alternate, so that one barrier a row is enough: a wave is at most one row ahead
+        const float mean = (float)(row_sum(dot, tpr, sm[turn]) / (double)cols);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int it = t + k * tpr;
+            const int64_t left = cols - (int64_t)it * 8;
+            const int valid = (int)(left < 8 ? left : 8);
+            if (valid > 0) {
+                float up[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) up[e] = HOLD ? uh[HOLD ? k : 0][e] : 0.f;
+                if constexpr (!HOLD) if (gh) mx_load8<DT, VEC>(gh, row * ldgh + it * 8, valid, up);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) up[e] = fmaf(rs, fmaf(-mean, xh[k][e], g[k][e]), up[e]);
+                mx_store8<DT, VEC>(dh, row * ldd + it * 8, valid, up);
+            }
+        }
+    }
+    if (part) {
+        const int64_t base = ((int64_t)blockIdx.x * slots + slot) * items * 8;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+            if (t + k * tpr < items) mx_store8<MX_F32, true>(part, base + (int64_t)(t + k * tpr) * 8, 8, acc[k]);
+    }
+}
+
+// dw[c] = sum over n rows of part[.][ld], 32 columns to a workgroup, 32 lanes down each column, added in a fixed order
+template <int WDT> __global__ __launch_bounds__(1024) void k_colsum(const float* __restrict__ part, int64_t ld, int n, void* __restrict__ dw, int64_t cols) {
+    __shared__ double sm[32][33];
+    const int c = threadIdx.x & 31, p = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    double s = 0;
+    if (col < cols)
+        for (int i = p; i < n; i += 32) s += (double)part[(int64_t)i * ld + col];
+    sm[p][c] = s;
+    __syncthreads();
+    if (p == 0 && col < cols) {
+        for (int i = 1; i < 32; ++i) s += sm[i][c];
+        if constexpr (WDT == MX_F32) ((float*)dw)[col] = (float)s;
+        else ((uint16_t*)dw)[col] = (uint16_t)mx_pair<WDT>((float)s, 0.f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+static inline bool mx_dt_ok(int dt) { return dt == MX_F32 || dt == MX_BF16 || dt == MX_F16; }
+static inline int mx_bytes(int dt) { return dt == MX_F32 ? 4 : 2; }
+// 16-byte accesses to rows of p: base, row pitch (elements) and length in whole eights
+static inline bool mx_vec(const void* p, int64_t ld, int dt, int64_t rows) {
+    return p == nullptr || ((uintptr_t)p % 16 == 0 && (rows <= 1 || ld * mx_bytes(dt) % 16 == 0));
+}
+static inline int64_t mx_blocks(int64_t cols) { return (cols + 31) / 32; }
+
+#define MX_DT(dt, ...)                                              \
+    switch (dt) {                                                   \
+        case MX_F32: { constexpr int DT = MX_F32; __VA_ARGS__ } break;   \
+        case MX_BF16: { constexpr int DT = MX_BF16; __VA_ARGS__ } break; \
+        default: { constexpr int DT = MX_F16; __VA_ARGS__ } break;       \
+    }
+
+template <int OP>
+static int mx_elem(const void* x, int64_t ldx, const void* gy, int64_t ldg, int dt, void* out, int64_t ldo, uint8_t* codes, int64_t ldc,
+                   uint8_t* scales, int64_t lds, int64_t rows, int64_t cols, int fmt, void* stream) {
+    const int64_t nb = mx_blocks(cols);
+    bool vec = cols % 8 == 0 && mx_vec(x, ldx, dt, rows) && mx_vec(gy, ldg, dt, rows) && mx_vec(out, ldo, dt, rows);
+    if (rows > 1 && cols % 32 == 0 && ldx == cols && (!gy || ldg == cols) && (!out || ldo == cols) &&
+        (!codes || (ldc == nb * (fmt == MX_FP4 ? 16 : 32) && lds == nb))) {
+        cols *= rows;                                                 // dense rows of whole blocks: one long row
+        rows = 1;
+    }
+    const int64_t items = mx_blocks(cols) * 4, total = rows * items;
+    // work per thread: one item where more would leave the 256 CUs without eight waves each, else 64 bytes of x in flight
+    const bool wide = total >= (int64_t)256 * 8 * 64 * 4;
+    hipStream_t st = (hipStream_t)stream;
+#define MX_GO(V, U)                                                                                                              \
+    do {                                                                                                                         \
+        const int64_t grid = (total + 256 * U - 1) / (256 * U);                                                                  \
+        if (grid > 0x7fffffff) return EDADM_EINVAL;                                                                              \
+        if (fmt == MX_FP4) k_mx_elem<DT, MX_FP4, OP, V, U><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
+        else k_mx_elem<DT, MX_FP8, OP, V, U><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
+    } while (0)
+    MX_DT(dt, {
+        if (!vec) MX_GO(false, 1);
+        else if (wide) MX_GO(true, (DT == MX_F32 ? 2 : 4));
+        else MX_GO(true, 1);
+    })
+#undef MX_GO
+    return edadm_launch_status();
+}
+
+static inline bool mx_fmt_ok(int fmt) { return fmt == MX_FP4 || fmt == MX_FP8; }
+// codes are read and written in pieces of 16 bytes a block half, the scale bytes one by one
+static inline bool mx_codes_ok(const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t cols, int fmt, int64_t rows) {
+    const int64_t nb = mx_blocks(cols), pitch = nb * (fmt == MX_FP4 ? 16 : 32);
+    return codes && scales && (uintptr_t)codes % 16 == 0 && ldc >= pitch && (rows <= 1 || ldc % 16 == 0) && lds >= nb;
+}
+
+extern "C" int edadm_mx_quantize(const void* x, int64_t ldx, int dt, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds,
+                                 int64_t rows, int64_t cols, int fmt, void* stream) {
+    if (rows < 0 || cols < 1 || !mx_dt_ok(dt) || !mx_fmt_ok(fmt)) return EDADM_EINVAL;
+    if (rows == 0) return 0;
+    if (!x || ldx < cols || !mx_codes_ok(codes, ldc, scales, lds, cols, fmt, rows)) return EDADM_EINVAL;
+    return mx_elem<MX_QUANT>(x, ldx, nullptr, 0, dt, nullptr, 0, codes, ldc, scales, lds, rows, cols, fmt, stream);
+}
+extern "C" int edadm_mx_fake_quant_fwd(const void* x, int64_t ldx, int dt, void* out, int64_t ldo, int64_t rows, int64_t cols, int fmt,
+                                       void* stream) {
+    if (rows < 0 || cols < 1 || !mx_dt_ok(dt) || !mx_fmt_ok(fmt)) return EDADM_EINVAL;
+    if (rows == 0) return 0;
+    if (!x || !out || ldx < cols || ldo < cols) return EDADM_EINVAL;
+    return mx_elem<MX_FAKE>(x, ldx, nullptr, 0, dt, out, ldo, nullptr, 0, nullptr, 0, rows, cols, fmt, stream);
+}
+extern "C" int edadm_mx_fake_quant_bwd(const void* gy, int64_t ldg, const void* x, int64_t ldx, int dt, void* gx, int64_t ldo, int64_t rows,
+                                       int64_t cols, int fmt, void* stream) {
+    if (rows < 0 || cols < 1 || !mx_dt_ok(dt) || !mx_fmt_ok(fmt)) return EDADM_EINVAL;
+    if (rows == 0) return 0;
+    if (!x || !gy || !gx || ldx < cols || ldg < cols || ldo < cols) return EDADM_EINVAL;
+    return mx_elem<MX_GRAD>(x, ldx, gy, ldg, dt, gx, ldo, nullptr, 0, nullptr, 0, rows, cols, fmt, stream);
+}
+extern "C" int edadm_mx_dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int fmt, void* out, int64_t ldo,
+                                   int dt, int64_t rows, int64_t cols, void* stream) {
+    if (rows < 0 || cols < 1 || !mx_dt_ok(dt) || !mx_fmt_ok(fmt)) return EDADM_EINVAL;
+    if (rows == 0) return 0;
+    if (!out || ldo < cols || !mx_codes_ok(codes, ldc, scales, lds, cols, fmt, rows)) return EDADM_EINVAL;
+    const bool vec = cols % 8 == 0 && mx_vec(out, ldo, dt, rows);
+    const int64_t nb = mx_blocks(cols);
+    if (rows > 1 && cols % 32 == 0 && ldo == cols && ldc == nb * (fmt == MX_FP4 ? 16 : 32) && lds == nb) {
+        cols *= rows;
+        rows = 1;
+    }
+    const int64_t items = mx_blocks(cols) * 4, total = rows * items;
+    const bool wide = total >= (int64_t)256 * 8 * 64 * 4;
+    hipStream_t st = (hipStream_t)stream;
+#define MX_GO(V, U)                                                                                                              \
+    do {                                                                                                                         \
+        const int64_t grid = (total + 256 * U - 1) / (256 * U);                                                                  \
+        if (grid > 0x7fffffff) return EDADM_EINVAL;                                                                              \
+        if (fmt == MX_FP4) k_mx_read<DT, MX_FP4, V, U><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items); \
+        else k_mx_read<DT, MX_FP8, V, U><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items);   \
+    } while (0)
+    MX_DT(dt, {
+        if (!vec) MX_GO(false, 1);
+        else if (wide) MX_GO(true, (DT == MX_F32 ? 2 : 4));
+        else MX_GO(true, 1);
+    })
+#undef MX_GO
+    return edadm_launch_status();
+}
+
+#define RMS_MAX_COLS 32768      // 1024 threads x 4 eights
+
+// threads per row and eights per thread: the fewest eights that keep a row within 1024 threads, more of them where there are
+// rows enough to fill the chip anyway (fewer waves, more loads in flight in each)
+static inline void rms_shape(int64_t rows, int64_t items, int* vpt, int* tpr) {
+    int v = rows >= 2048 ? 2 : 1;
+    if (items <= 64 * 4 && rows >= 2048) v = items <= 64 ? 1 : items <= 128 ? 2 : 4;
+    while ((items + v - 1) / v > 1024) v *= 2;
+    *vpt = v;
+    *tpr = (int)(((items + v - 1) / v + 63) / 64 * 64);
+}
+
+extern "C" int64_t edadm_rmsnorm_max_cols(void) { return RMS_MAX_COLS; }
+
+extern "C" int edadm_rmsnorm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, int dt, const void* weight, int weight_f32,
+                                 void* h, int64_t ldh, float* rstd, void* out, int64_t ldo, uint8_t* scales, int64_t lds, int64_t rows,
+                                 int64_t cols, double eps, int fmt, int fake, void* stream) {
+    if (rows < 0 || cols < 1 || cols > RMS_MAX_COLS || !mx_dt_ok(dt) || !(fmt == 0 || mx_fmt_ok(fmt))) return EDADM_EINVAL;
+    if (rows == 0) return 0;
+    if (!x || !weight || !out || ldx < cols || (res && (!h || ldr < cols || ldh < cols)) || !(eps >= 0.0)) return EDADM_EINVAL;
+    const bool codes = fmt && !fake;
+    if (codes ? !mx_codes_ok(out, ldo, scales, lds, cols, fmt, rows) : ldo < cols) return EDADM_EINVAL;
+    const bool vec = cols % 8 == 0 && mx_vec(x, ldx, dt, rows) && mx_vec(res, ldr, dt, rows) && mx_vec(res ? h : nullptr, ldh, dt, rows) &&
+                     mx_vec(weight, 0, dt, 1) && (codes || mx_vec(out, ldo, dt, rows));
+    const int64_t items = mx_blocks(cols) * 4;
+    int vpt, tpr;
+    rms_shape(rows, items, &vpt, &tpr);
+    const int mode = fake && fmt ? 16 + fmt : fmt, per = tpr == 64 ? 4 : 1;
+    const int64_t grid = (rows + per - 1) / per;
+    if (grid > 0x7fffffff) return EDADM_EINVAL;
+    hipStream_t st = (hipStream_t)stream;
+#define RMS_GO(W, P, V) k_rmsnorm<DT, W, P, V><<<(unsigned)grid, tpr * per, 0, st>>>(x, ldx, res, ldr, weight, h, ldh, rstd, out, ldo, scales, lds, rows, cols, (int)items, eps, mode, tpr)
+#define RMS_V(W, V) do { if (vpt == 1) RMS_GO(W, 1, V); else if (vpt == 2) RMS_GO(W, 2, V); else RMS_GO(W, 4, V); } while (0)
+    MX_DT(dt, {
+        if (weight_f32 || dt == MX_F32) { if (vec) RMS_V(true, true); else RMS_V(true, false); }
+        else { if (vec) RMS_V(false, true); else RMS_V(false, false); }
+    })
+#undef RMS_V
+#undef RMS_GO
+    return edadm_launch_status();
+}
+
+// rows of `part`: as many workgroups as the chip holds at once, four row slots each where a row is one wave
+static inline int rms_bwd_grid(int64_t rows, int tpr) {
+    const int64_t want = tpr == 64 ? (rows + 3) / 4 : rows, most = tpr == 64 ? 512 : tpr <= 320 ? 768 : tpr <= 512 ? 512 : 256;
+    return (int)(want < most ? want : most);
+}
+extern "C" int64_t edadm_rmsnorm_bwd_ws_floats(int64_t rows, int64_t cols) {
+    if (rows < 1 || cols < 1 || cols > RMS_MAX_COLS) return 0;
+    int vpt, tpr;
+    const int64_t items = mx_blocks(cols) * 4;
+    rms_shape(rows, items, &vpt, &tpr);
+    return (int64_t)rms_bwd_grid(rows, tpr) * (tpr == 64 ? 4 : 1) * items * 8;
+}
+extern "C" int edadm_rmsnorm_bwd(const void* gy, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, int dt,
+                                 const float* rstd, const void* weight, int weight_f32, void* dh, int64_t ldd, void* dw, float* ws,
+                                 int64_t rows, int64_t cols, int fmt, void* stream) {
+    if (rows < 0 || cols < 1 || cols > RMS_MAX_COLS || !mx_dt_ok(dt) || !(fmt == 0 || mx_fmt_ok(fmt))) return EDADM_EINVAL;
+    if ((dw && !ws) || (uintptr_t)ws % 16) return EDADM_EINVAL;
+    if (rows == 0 && !dw) return 0;
+    if (rows && (!gy || !h || !rstd || !weight || !dh || ldg < cols || ldh < cols || ldd < cols || (gh && ldgh < cols))) return EDADM_EINVAL;
+    const bool vec = cols % 8 == 0 && mx_vec(gy, ldg, dt, rows) && mx_vec(gh, ldgh, dt, rows) && mx_vec(h, ldh, dt, rows) &&
+                     mx_vec(weight, 0, dt, 1) && mx_vec(dh, ldd, dt, rows);
+    const int64_t items = mx_blocks(cols) * 4;
+    int vpt, tpr;
+    rms_shape(rows, items, &vpt, &tpr);
+    const int per = tpr == 64 ? 4 : 1, grid = rms_bwd_grid(rows, tpr);
+    hipStream_t st = (hipStream_t)stream;
+    const bool wf32 = weight_f32 || dt == MX_F32;
+#define RMS_GO(W, P, V) k_rmsnorm_bwd<DT, W, P, V><<<grid, tpr * per, 0, st>>>(gy, ldg, gh, ldgh, h, ldh, rstd, weight, dh, ldd, dw ? ws : nullptr, rows, cols, (int)items, fmt, tpr)
+#define RMS_V(W, V) do { if (vpt == 1) RMS_GO(W, 1, V); else if (vpt == 2) RMS_GO(W, 2, V); else RMS_GO(W, 4, V); } while (0)
+    if (rows) MX_DT(dt, {
+        if (wf32) { if (vec) RMS_V(true, true); else RMS_V(true, false); }
+        else { if (vec) RMS_V(false, true); else RMS_V(false, false); }
+    })
+#undef RMS_V
+#undef RMS_GO
+    if (dw) {
+        const unsigned g = (unsigned)((cols + 31) / 32);
+        const int n = rows ? grid * per : 0;
+        if (wf32) k_colsum<MX_F32><<<g, 1024, 0, st>>>(ws, items * 8, n, dw, cols);
+        else if (dt == MX_BF16) k_colsum<MX_BF16><<<g, 1024, 0, st>>>(ws, items * 8, n, dw, cols);
+        else k_colsum<MX_F16><<<g, 1024, 0, st>>>(ws, items * 8, n, dw, cols);
+    }
+    return edadm_launch_status();
+}

@@ -1,0 +1,161 @@
+// Microscaled formats on gfx950: 32 consecutive elements of a row share one power-of-two scale.  A lane works on 8 consecutive
+// elements, so a block of 32 is the four lanes of a DPP quad and its maximum is two quad permutations away.
+#pragma once
+#include "common.h"
+
+#define MX_F32 0
+#define MX_BF16 1
+#define MX_F16 2
+#define MX_FP4 4   // e2m1, two to a byte, the first in the low nibble
+#define MX_FP8 8   // e4m3
+
+typedef float mx_f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 mx_h2 __attribute__((ext_vector_type(2)));
+typedef short mx_s2 __attribute__((ext_vector_type(2)));
+
+template <int DT> struct mx_size { static constexpr int v = DT == MX_F32 ? 4 : 2; };
+
+__device__ __forceinline__ float mx_lo(uint32_t u, int dt) {
+    return dt == MX_BF16 ? __builtin_bit_cast(float, u << 16) : (float)__builtin_bit_cast(mx_h2, u)[0];
+}
+__device__ __forceinline__ float mx_hi(uint32_t u, int dt) {
+    return dt == MX_BF16 ? __builtin_bit_cast(float, u & 0xffff0000u) : (float)__builtin_bit_cast(mx_h2, u)[1];
+}
+// two floats -> two 16-bit values, rounded to nearest even
+template <int DT> __device__ __forceinline__ uint32_t mx_pair(float a, float b) {
+    const mx_f2 v = {a, b};
+    if constexpr (DT == MX_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_b2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_h2));
+}
+
+// 8 elements at element offset `at`; VEC: 16-byte loads (the host has checked alignment and that rows are whole eights), else
+// one by one, `valid` (<= 8, may be <= 0) of them, the others 0
+template <int DT, bool VEC> __device__ __forceinline__ void mx_load8(const void* p, int64_t at, int valid, float (&v)[8]) {
+    if constexpr (VEC) {
+        const uint4* q = (const uint4*)((const char*)p + at * mx_size<DT>::v);
+        if constexpr (DT == MX_F32) {
+            const uint4 a = q[0], b = q[1];
+            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+        } else {
+            const uint4 a = q[0];
+            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[2 * e] = mx_lo(u[e], DT); v[2 * e + 1] = mx_hi(u[e], DT); }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = 0.f;
+            if (e < valid) {
+                if constexpr (DT == MX_F32) v[e] = ((const float*)p)[at + e];
+                else v[e] = mx_lo(((const uint16_t*)p)[at + e], DT);
+            }
+        }
+    }
+}
+template <int DT, bool VEC> __device__ __forceinline__ void mx_store8(void* p, int64_t at, int valid, const float (&v)[8]) {
+    if constexpr (VEC) {
+        uint4* q = (uint4*)((char*)p + at * mx_size<DT>::v);
+        if constexpr (DT == MX_F32) {
+            q[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            q[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+        } else {
+            q[0] = make_uint4(mx_pair<DT>(v[0], v[1]), mx_pair<DT>(v[2], v[3]), mx_pair<DT>(v[4], v[5]), mx_pair<DT>(v[6], v[7]));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < valid) {
+                if constexpr (DT == MX_F32) ((float*)p)[at + e] = v[e];
+                else ((uint16_t*)p)[at + e] = (uint16_t)mx_pair<DT>(v[e], 0.f);
+            }
+    }
+}
+// round to the type a value is stored in, in place
+template <int DT> __device__ __forceinline__ void mx_round8(float (&v)[8]) {
+    if constexpr (DT != MX_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u = mx_pair<DT>(v[2 * e], v[2 * e + 1]);
+            v[2 * e] = mx_lo(u, DT);
+            v[2 * e + 1] = mx_hi(u, DT);
+        }
+    }
+}
+
+// The block's biased exponent byte: floor(log2 max|x|) - emax clamped below at 0 (2^-127), read off the exponent field of the
+// largest magnitude (magnitudes of floats order like their bits, infinities and NaN above every number): 255, which stands for
+// NaN, where the block holds one of those.  All four lanes of a quad call this together.
+template <int FMT> __device__ __forceinline__ uint32_t mx_block_exp(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    const int b = (int)(m >> 23) - (FMT == MX_FP4 ? 2 : 8);
+    return m >= 0x7f800000u ? 255u : (uint32_t)max(b, 0);
+}
+__device__ __forceinline__ float mx_scale(uint32_t b) {
+    return b == 0 ? __uint_as_float(0x00400000u) : b == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(b << 23);
+}
+
+// 8 scaled elements -> codes (fp4: 8 nibbles in x; fp8: 8 bytes in x, y).  v_cvt_scalef32_* divide by the scale and round to
+// nearest even, subnormal elements included; the e2m1 form saturates at 6, the e4m3 form turns what would round past 448 into
+// NaN, so it is clamped first.  A block of exponent 255 gets zero codes: 0 * NaN = NaN wherever it is read.
+template <int FMT> __device__ __forceinline__ uint2 mx_encode8(const float (&v)[8], uint32_t b, float s) {
+    uint2 c = make_uint2(0, 0);
+    if constexpr (FMT == MX_FP4) {
+        c.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c.x, v[0], v[1], s, 0);
+        c.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c.x, v[2], v[3], s, 1);
+        c.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c.x, v[4], v[5], s, 2);
+        c.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c.x, v[6], v[7], s, 3);
+    } else {
+        const float top = 448.f * s;
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = clampf(v[e], -top, top);
+        mx_s2 x = {0, 0}, y = {0, 0};
+        x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, q[0], q[1], s, false);
+        x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, q[2], q[3], s, true);
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(y, q[4], q[5], s, false);
+        y = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(y, q[6], q[7], s, true);
+        c = make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
+    }
+    return b == 255 ? make_uint2(0, 0) : c;
+}
+// codes -> the values they stand for.  The conversion itself runs at scale 1 and an IEEE product applies the scale, so that
+// values below 2^-126 come out as the subnormals they are.
+template <int FMT> __device__ __forceinline__ void mx_decode8(uint2 c, float s, float (&v)[8]) {
+    mx_f2 p[4];
+    if constexpr (FMT == MX_FP4) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, 1.f, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, 1.f, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, 1.f, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, 1.f, 3);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, false);
+        p[1] = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, true);
+        p[2] = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, false);
+        p[3] = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, true);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p[e >> 1][e & 1] * s;
+}
+// v = what its quantised form stands for
+template <int FMT> __device__ __forceinline__ void mx_fake8(float (&v)[8]) {
+    const uint32_t b = mx_block_exp<FMT>(v);
+    const float s = mx_scale(b);
+    mx_decode8<FMT>(mx_encode8<FMT>(v, b, s), s, v);
+}
+// the largest magnitude the block's scale represents: a gradient passes where |x| does not exceed it (never where it is NaN)
+template <int FMT> __device__ __forceinline__ float mx_top(const float (&v)[8]) {
+    return (FMT == MX_FP4 ? 6.f : 448.f) * mx_scale(mx_block_exp<FMT>(v));
+}
+// store a lane's codes and, from the first lane of its quad, the block's scale byte.  item: index of the eight in its row
+template <int FMT> __device__ __forceinline__ void mx_put(uint8_t* codes, uint8_t* scales, int64_t item, uint2 c, uint32_t b) {
+    if constexpr (FMT == MX_FP4) *(uint32_t*)(codes + item * 4) = c.x;
+    else *(uint2*)(codes + item * 8) = c;
+    if ((item & 3) == 0) scales[item >> 2] = (uint8_t)b;
+}

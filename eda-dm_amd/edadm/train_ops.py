@@ -8,6 +8,7 @@ import ctypes
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import lib, ops
 from .ops import _pf, _stream
@@ -232,3 +233,53 @@ class _BmmNtFn(torch.autograd.Function):
 def bmm_nt(a, b, alpha=1.0):
     """Batched a . b^T with autograd: a [Z, M, K], b [Z, N, K] -> [Z, M, N]."""
     return _BmmNtFn.apply(a, b, alpha)
+
+
+# ----------------------------------------------------------------------------- microscaled fake quantisation, root-mean-square norm
+class _MxFakeQuantFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, fmt):
+        ctx.save_for_backward(x)
+        ctx.fmt = fmt
+        return ops.mx_fake_quant_fwd(x, fmt)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        (x,) = ctx.saved_tensors
+        return ops.mx_fake_quant_bwd(gy, x, ctx.fmt), None
+
+
+def mx_fake_quant(x, fmt):
+    """The values x's microscaled form stands for, in x's type, straight-through: the gradient passes where |x| is at most the largest
+    value its block's scale represents (6 / 448 times the scale) and is 0 where the quantiser clips, as UniformAffineQuantizer's is
+    (quant_layer.py:266-276); the scale itself gets none."""
+    return _MxFakeQuantFn.apply(x, fmt)
+
+
+class _RmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, fmt, residual):
+        y, h, rstd = ops.rmsnorm_fwd(x, weight, eps, fmt, residual, fake=fmt is not None, want_rstd=True)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.fmt, ctx.two = fmt, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.two else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if gy is None:                                     # only the stream went on: its gradient passes through the addition
+            return (gh if need[0] else None, torch.zeros_like(weight) if need[1] else None, None, None,
+                    gh if ctx.two and need[4] else None)
+        dh, dw = ops.rmsnorm_bwd(gy, gh, h, rstd, weight, ctx.fmt, need_dw=need[1])
+        return dh if need[0] else None, dw, None, None, dh if ctx.two and need[4] else None
+
+
+def rms_norm(x, weight, eps, fmt=None, residual=None):
+    """Root-mean-square norm over the last dimension: y = h / sqrt(mean(h^2) + eps) * weight with h = x + residual rounded to x's type; y in
+    x's type, under `fmt` ('mxfp8' / 'mxfp4') the values its microscaled form stands for (straight-through as mx_fake_quant).  Returns y,
+    or (y, h) with a residual.  Gradients of x, residual and weight."""
+    return _RmsNormFn.apply(x, weight, eps, fmt, residual)

@@ -527,6 +527,50 @@ int edadm_transpose_batched_f32(const float* x, float* out, int64_t Z, int64_t R
 int edadm_tdac_pair_scores(const float* feats, int64_t T, int64_t B, int64_t C, int64_t P, float eps, float* mse, float* cosdis,
                            void* stream);
 
+/* ---- Microscaled (MX) formats: 4-bit weights and 4- or 8-bit activations with a shared power-of-two scale per 32 elements --------
+ * The format the block-scaled matrix instructions of gfx950 read.  A row is cut into blocks of 32 elements; block j of a row holds
+ * 32 codes and one byte b: value = element * 2^(b - 127), with b - 127 = max(floor(log2 max|x|) - emax, -127) (Open Compute MX
+ * conversion; b = 255, every value NaN, where the block holds an infinity or a NaN).  Elements are rounded to nearest even and saturate.
+ *   fmt 4: e2m1 (emax 2, largest 6), two codes to a byte, the first element in the low nibble: 16 bytes a block
+ *   fmt 8: e4m3 (emax 8, largest 448): 32 bytes a block
+ * A row whose length is no multiple of 32 ends in a block filled up with zero codes.  codes: 16-byte aligned, row pitch ldc in BYTES
+ * (a multiple of 16); scales: one byte a block, row pitch lds in bytes, any alignment.  dt: 0 fp32, 1 bf16, 2 fp16; row pitches of
+ * such tensors (ldx, ...) in elements, any alignment.  They stand next to the uniform quantisers of the calibration graph and the
+ * sampling path (quant_layer.py:266-276, :406-437): the same places of a transformer block, a scale per 32 elements instead of
+ * one per tensor or channel. */
+int edadm_mx_quantize(const void* x, int64_t ldx, int dt, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds,
+                      int64_t rows, int64_t cols, int fmt, void* stream);
+int edadm_mx_dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int fmt, void* out, int64_t ldo,
+                        int dt, int64_t rows, int64_t cols, void* stream);
+/* the calibration graph's form: out = what the quantised x stands for, in x's type; backward gx = gy where |x| is at most the
+ * largest value its block's scale represents (6 or 448 times the scale), 0 elsewhere and in blocks that hold an infinity or NaN */
+int edadm_mx_fake_quant_fwd(const void* x, int64_t ldx, int dt, void* out, int64_t ldo, int64_t rows, int64_t cols, int fmt,
+                            void* stream);
+int edadm_mx_fake_quant_bwd(const void* gy, int64_t ldg, const void* x, int64_t ldx, int dt, void* gx, int64_t ldo, int64_t rows,
+                            int64_t cols, int fmt, void* stream);
+/* Root-mean-square norm with the residual's addition (the place of attention.py:222-242's LayerNorms in networks that use the
+ * root mean square): h = x + res rounded to dt (res NULL: h = x, nothing stored), rstd = 1 / sqrt(mean(h^2) + eps), y = (h rstd)
+ * weight with both products in fp32.  fmt 0: out = y in dt; fmt 4 / 8 and fake 0: out = codes (ldo in bytes), scales; fake 1: out =
+ * what the quantised y stands for, in dt.  weight: contiguous [cols], fp32 (weight_f32) or dt.  rstd [rows] (may be NULL) for the backward:
+ *   g = gy where |y| was at most its block's largest value (everywhere for fmt 0), 0 elsewhere;  xh = h rstd
+ *   dh = gh + rstd (g weight - xh mean(g weight xh))  in dt = the gradient of x and of res;  dw = sum over rows g xh  in weight's type
+ * (gh: the gradient arriving at h, may be NULL; dw NULL: not computed).  ws: edadm_rmsnorm_bwd_ws_floats floats, 16-byte
+ * aligned; sums are added in one fixed order.  1 <= cols <= edadm_rmsnorm_max_cols(). */
+int64_t edadm_rmsnorm_max_cols(void);
+int edadm_rmsnorm_fwd(const void* x, int64_t ldx, const void* res, int64_t ldr, int dt, const void* weight, int weight_f32,
+                      void* h, int64_t ldh, float* rstd, void* out, int64_t ldo, uint8_t* scales, int64_t lds, int64_t rows,
+                      int64_t cols, double eps, int fmt, int fake, void* stream);
+int64_t edadm_rmsnorm_bwd_ws_floats(int64_t rows, int64_t cols);
+int edadm_rmsnorm_bwd(const void* gy, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, int dt,
+                      const float* rstd, const void* weight, int weight_f32, void* dh, int64_t ldd, void* dw, float* ws,
+                      int64_t rows, int64_t cols, int fmt, void* stream);
+/* out[m][n] = sum_k A[m][k] W[n][k] (+ bias[n], fp32) over microscaled operands: A in afmt 8 or 4, W in format 4, both as
+ * edadm_mx_quantize writes them, fp32 accumulation, out in odt (0 fp32, 1 bf16, 2 fp16) with row pitch ldo elements.  The counterpart
+ * of edadm_qgemm_i8 / edadm_qgemm_w4 (quant_layer.py:406-437 at inference). */
+int edadm_mx_gemm(const uint8_t* A, int64_t lda, const uint8_t* As, int64_t ldas, int afmt, const uint8_t* W, int64_t ldw,
+                  const uint8_t* Ws, int64_t ldws, int64_t M, int64_t N, int64_t K, const float* bias, void* out, int64_t ldo,
+                  int odt, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

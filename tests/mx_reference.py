@@ -1,0 +1,78 @@
+"""The microscaled formats, the root-mean-square norm and the product restated on the CPU in 64 bits, for the tests: element tables and
+comparisons with the midpoints between them, no bit tricks shared with the kernels."""
+import torch
+
+EMAX = {"mxfp4": 2, "mxfp8": 8}
+TOP = {"mxfp4": 6.0, "mxfp8": 448.0}
+E2M1 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+# the 127 finite magnitudes of e4m3 in the order of their codes: (1 + m/8) 2^(e - 7), subnormal m/8 2^-6
+E4M3 = torch.tensor([(m / 8 if e == 0 else 1 + m / 8) * 2.0 ** (max(e, 1) - 7) for e in range(16) for m in range(8)][:127], dtype=torch.float64)
+TABLE = {"mxfp4": E2M1, "mxfp8": E4M3}
+
+
+def nearest(v, fmt):
+    """code of the element nearest to each magnitude in v (64 bits, finite); a tie goes to the even code, what is past the last element
+    to the last"""
+    t = TABLE[fmt]
+    mid = (t[1:] + t[:-1]) / 2
+    below, above = torch.bucketize(v, mid), torch.bucketize(v, mid, right=True)      # they differ exactly on a midpoint
+    return torch.where(below % 2 == 0, below, above)
+
+
+def blocks(x):
+    rows, cols = x.shape
+    b = torch.zeros(rows, -(-cols // 32) * 32, dtype=torch.float64)
+    b[:, :cols] = x.double()
+    return b.reshape(rows, -1, 32)
+
+
+def quantize(x, fmt):
+    """x [rows, cols] -> (codes uint8 [rows, blocks * 32] one to an element, biased exponents [rows, blocks], inside [rows, cols])"""
+    rows, cols = x.shape
+    b = blocks(x)
+    top = b.abs().amax(-1)
+    bad = ~torch.isfinite(b).all(-1)
+    # floor(log2 top) by comparison with every power of two a 32-bit number reaches
+    powers = 2.0 ** torch.arange(-149, 128, dtype=torch.float64)
+    e = torch.bucketize(torch.where(bad, torch.ones_like(top), top), powers, right=True) - 1 - 149 - EMAX[fmt]
+    byte = e.clamp_min(-127) + 127
+    byte = torch.where(top > 0, byte, torch.zeros_like(byte))
+    byte = torch.where(bad, torch.full_like(byte, 255), byte)
+    scale = 2.0 ** (byte.double() - 127)
+    v = torch.where(bad.unsqueeze(-1), torch.zeros_like(b), b / scale.unsqueeze(-1))
+    code = nearest(v.abs(), fmt).to(torch.uint8) | (torch.signbit(v).to(torch.uint8) << (3 if fmt == "mxfp4" else 7))
+    code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code)
+    inside = (b.abs() <= TOP[fmt] * scale.unsqueeze(-1)) & ~bad.unsqueeze(-1)
+    return code.reshape(rows, -1), byte.to(torch.uint8), inside.reshape(rows, -1)[:, :cols]
+
+
+def pack(code, fmt):
+    return code if fmt == "mxfp8" else code[:, 0::2] | (code[:, 1::2] << 4)
+
+
+def values(code, byte, cols, fmt):
+    """one code to an element -> the values in 64 bits"""
+    bit = 3 if fmt == "mxfp4" else 7
+    v = TABLE[fmt][(code & ((1 << bit) - 1)).long()] * torch.where(code >> bit == 1, -1.0, 1.0).double()
+    scale = torch.where(byte == 255, torch.tensor(float("nan"), dtype=torch.float64), 2.0 ** (byte.double() - 127))
+    return (v.reshape(v.shape[0], -1, 32) * scale.unsqueeze(-1)).reshape(v.shape[0], -1)[:, :cols]
+
+
+def fake(x, fmt):
+    """(values in 64 bits, inside)"""
+    code, byte, inside = quantize(x, fmt)
+    return values(code, byte, x.shape[1], fmt), inside
+
+
+def rms(x, res, weight, eps, dtype):
+    """(h in its type, rstd 64 bits, y in 32 bits as the operator defines it: rstd and both products rounded to 32 bits)"""
+    h = x if res is None else (x.double() + res.double()).to(dtype)
+    rstd = 1 / torch.sqrt((h.double() ** 2).mean(-1, keepdim=True) + eps)
+    y = ((h.double() * rstd.float().double()).float().double() * weight.double()).float()
+    return h, rstd, y
+
+
+def rms_grads(gy, gh, h, rstd, weight, inside):
+    g, xh, w = gy.double() * inside, h.double() * rstd, weight.double()
+    d = rstd * (g * w - xh * (g * w * xh).mean(-1, keepdim=True))
+    return (d if gh is None else d + gh.double()), (g * xh).sum(0)

@@ -1,0 +1,513 @@
+"""-m gpu: the microscaled operators (csrc/mx.hip, csrc/mx_gemm.hip through edadm.ops / edadm.train_ops) against tests/mx_reference.py
+in 64 bits.  Codes, scales and the values they stand for are compared bit for bit; computed numbers within the tolerance derived next
+to each check."""
+import pytest
+import torch
+
+import mx_reference as R
+
+pytestmark = pytest.mark.gpu
+FMTS = ("mxfp8", "mxfp4")
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+HALF = {t: torch.finfo(t).eps / 2 for t in DTYPES}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a device"
+    from edadm import ops as _ops
+    return _ops
+
+
+@pytest.fixture(scope="module")
+def tops():
+    from edadm import train_ops
+    return train_ops
+
+
+def data(shape, dtype, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * torch.exp(spread * torch.randn(shape[-1], generator=g))).to(dtype)
+
+
+def same(a, b):
+    a, b = a.detach().cpu(), b.detach().cpu()
+    assert a.shape == b.shape and a.dtype == b.dtype, (a.shape, b.shape, a.dtype, b.dtype)
+    if a.dtype.is_floating_point:
+        assert torch.equal(torch.isnan(a), torch.isnan(b))
+        a, b = torch.nan_to_num(a, 0.0, 1e38, -1e38), torch.nan_to_num(b, 0.0, 1e38, -1e38)
+    assert torch.equal(a, b), int((a != b).sum())
+
+
+def check_codes(q, x2d, fmt):
+    code, byte, _ = R.quantize(x2d, fmt)
+    same(q.scales.reshape(byte.shape), byte)
+    same(q.codes.reshape(x2d.shape[0], -1), R.pack(code, fmt))
+    return code, byte
+
+
+# ------------------------------------------------------------------------------------------------ quantisation and its inverse
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 31), (1, 32), (3, 33), (5, 64), (7, 100), (2, 8), (33, 1000), (1, 4096), (300, 4096), (1027, 260)])
+def test_quantize_and_back(ops, fmt, dtype, shape):
+    x = data(shape, dtype, sum(shape))
+    q = ops.mx_quantize(x.cuda(), fmt)
+    assert q.shape == x.shape and q.fmt == fmt
+    code, byte = check_codes(q, x, fmt)
+    v = R.values(code, byte, shape[1], fmt)
+    for out in DTYPES:
+        same(ops.mx_dequantize(q, out), v.to(out))               # one rounding from 64 bits
+    same(ops.mx_fake_quant_fwd(x.cuda(), fmt), v.to(dtype))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_every_16_bit_value_under_a_fixed_scale(ops, fmt):
+    """All finite bf16 and fp16 magnitudes up to the block's largest, ties among them, in blocks whose first element sets the scale:
+    2^0, the smallest scale and a large one."""
+    for dtype in (torch.bfloat16, torch.float16):
+        v = torch.arange(0, 65536, dtype=torch.int32).to(torch.int16).view(dtype).float()
+        v = v[torch.isfinite(v)]
+        for top in (4.0 if fmt == "mxfp4" else 256.0, 7.0 if fmt == "mxfp4" else 500.0):
+            for power in (0, -120, 100):
+                t = v[v.abs() <= top]
+                t = torch.nn.functional.pad(t, (0, -t.numel() % 31)).reshape(-1, 31)
+                x = torch.cat([torch.full((t.shape[0], 1), top), t], 1).double() * 2.0 ** power
+                x = x.float()
+                q = ops.mx_quantize(x.cuda(), fmt)
+                check_codes(q, x, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_extremes(ops, fmt):
+    inf, nan = float("inf"), float("nan")
+    x = torch.zeros(12, 64)
+    x[1, 3] = 1e-45                                              # the smallest subnormal
+    x[2, :32] = torch.linspace(-1e-38, 1e-38, 32)                # subnormals
+    x[3, 7], x[3, 40] = inf, 1.0                                 # one block infinite, the next one not
+    x[4, 9], x[4, 41] = nan, 2.0
+    x[5, 0], x[5, 1] = 3.4028234e38, -3.4028234e38               # the largest number, clipped
+    x[6, :] = -0.0
+    x[7, 31], x[7, 32] = 1.0, 1.9999999
+    x[8, :32] = 2.0 ** -126
+    x[9, 0], x[9, 1] = 2.0 ** 127, 1.0
+    x[10, :] = torch.randn(64, generator=torch.Generator().manual_seed(1)) * 2.0 ** -130
+    x[11, 63] = -inf
+    q = ops.mx_quantize(x.cuda(), fmt)
+    code, byte = check_codes(q, x, fmt)
+    v = R.values(code, byte, 64, fmt)
+    for out in DTYPES:
+        same(ops.mx_dequantize(q, out), v.to(out))
+    same(ops.mx_fake_quant_fwd(x.cuda(), fmt), v.float())
+    gy = torch.ones_like(x)
+    same(ops.mx_fake_quant_bwd(gy.cuda(), x.cuda(), fmt), R.fake(x, fmt)[1].float())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(ops, fmt, dtype):
+    base = data((40, 200), dtype, 3).cuda()
+    for name, x in (("columns", base[:, 8:136]), ("odd start", base[:, 3:131]), ("odd length", base[:, 1:100]), ("rows", base[::3]),
+                    ("transposed", base.t()), ("3-D", base.reshape(5, 8, 200)[:, ::2, 16:80]), ("expanded", base[:1].expand(6, 200)),
+                    ("one column", base[:, 5:6]), ("vector", base[7]), ("offset", base.reshape(-1)[1:1 + 32 * 64].reshape(32, 64))):
+        q = ops.mx_quantize(x, fmt)
+        x2 = x.cpu().reshape(-1, x.shape[-1])
+        code, byte = check_codes(q, x2, fmt)
+        v = R.values(code, byte, x.shape[-1], fmt).reshape(x.shape)
+        same(ops.mx_dequantize(q, dtype), v.to(dtype))
+        same(ops.mx_fake_quant_fwd(x, fmt), v.to(dtype))
+        g = data(tuple(x.shape), dtype, 4)
+        same(ops.mx_fake_quant_bwd(g.cuda(), x, fmt), g * R.fake(x2, fmt)[1].reshape(x.shape))
+    q = ops.mx_quantize(base[:0], fmt)
+    assert q.shape == (0, 200) and ops.mx_dequantize(q).shape == (0, 200) and ops.mx_fake_quant_fwd(base[:0], fmt).shape == (0, 200)
+    # a tensor of codes cut out of a larger one: rows apart, scales of any alignment
+    q = ops.mx_quantize(base[:, :192], fmt)
+    for rows in (slice(1, None, 2), slice(5, 6)):
+        p = ops.MXTensor(q.codes[rows], q.scales[rows], 192, fmt)
+        same(ops.mx_dequantize(p, dtype), ops.mx_dequantize(q, dtype)[rows])
+    wide = torch.zeros(40, 7 + q.codes.shape[1], dtype=torch.uint8, device="cuda")
+    wide[:, 7:] = q.codes
+    same(ops.mx_dequantize(ops.MXTensor(wide[:, 7:], q.scales, 192, fmt), dtype), ops.mx_dequantize(q, dtype))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (6, 45), (17, 512), (3, 5, 96), (513, 1024)])
+def test_fake_quant_gradient(tops, fmt, dtype, shape):
+    x, gy = data(shape, dtype, 11), data(shape, dtype, 12)
+    leaf = x.cuda().requires_grad_(True)
+    y = tops.mx_fake_quant(leaf, fmt)
+    (gx,) = torch.autograd.grad(y, leaf, gy.cuda())
+    v, inside = R.fake(x.reshape(-1, shape[-1]), fmt)
+    same(y, v.reshape(shape).to(dtype))
+    same(gx, torch.where(inside.reshape(shape), gy, torch.zeros_like(gy)))
+    if x.numel() > 1000:
+        assert 0 < int((~inside).sum()) < inside.numel() // 8    # some elements are clipped, few
+
+
+def test_rows_past_two_gigabytes(ops):
+    """offsets past 2^31 elements and 2^32 bytes: the first and last rows of a tensor that long, dense and strided, read and written"""
+    rows, cols = 140_000, 16_640
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    some = data((4, cols), torch.bfloat16, 5)
+    at = [0, 1, rows - 2, rows - 1]
+    x[at] = some.cuda()
+    for fmt in FMTS:
+        q = ops.mx_quantize(x, fmt)
+        code, byte, inside = R.quantize(some, fmt)
+        same(q.codes[at], R.pack(code, fmt))
+        same(q.scales[at], byte)
+        v = R.values(code, byte, cols, fmt).to(torch.bfloat16)
+        y = ops.mx_dequantize(q, torch.bfloat16)
+        same(y[at], v)
+        assert int(torch.count_nonzero(y[2:-2:1000])) == 0
+        del q, y
+        q = ops.mx_quantize(x[:, 5:], fmt)                       # unaligned rows: one by one
+        code, byte, _ = R.quantize(some[:, 5:], fmt)
+        same(q.codes[at], R.pack(code, fmt))
+        del q
+
+
+# ------------------------------------------------------------------------------------------------ root-mean-square norm
+SHAPES = [(1, 1), (1, 33), (3, 8), (2, 40), (5, 384), (9, 1000), (4, 2048), (3, 4096), (2, 8192), (2, 16384), (2, 20000), (1, 32768), (2100, 320),
+          (2050, 640), (2049, 1280), (2048, 2560), (4, 6, 96)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm(ops, shape, dtype, residual):
+    x, res = data(shape, dtype, 21), data(shape, dtype, 22) if residual else None
+    cols = shape[-1]
+    for wdt in {torch.float32, dtype}:
+        w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(2))).to(wdt)
+        x2, r2 = x.reshape(-1, cols), None if res is None else res.reshape(-1, cols)
+        h, rstd, y = R.rms(x2, r2, w, 1e-6, dtype)
+        args = (x.cuda(), w.cuda(), 1e-6)
+        kw = {"residual": None if res is None else res.cuda()}
+        got, gh, grstd = ops.rmsnorm_fwd(*args, want_rstd=True, **kw)
+        same(gh.reshape(h.shape), h)
+        same(grstd, rstd.reshape(-1).float())                    # summed in 64 bits, rounded once
+        same(got.reshape(h.shape), y.to(dtype))
+        for fmt in FMTS:
+            q, gh = ops.rmsnorm_mx(*args, fmt, **kw)
+            assert q.shape == x.shape
+            check_codes(q, y, fmt)
+            same(gh.reshape(h.shape), h)
+            got, _, _ = ops.rmsnorm_fwd(*args, fmt, fake=True, **kw)
+            same(got.reshape(h.shape), R.fake(y, fmt)[0].to(dtype))
+
+
+def test_rmsnorm_odd_rows(ops):
+    """rows of zeros (with and without eps), of one huge and of tiny numbers, with an infinity, with a NaN; strided and unaligned rows"""
+    x = data((8, 200), torch.float32, 31)
+    x[0] = 0
+    x[1] *= 1e30
+    x[2] *= 1e-30
+    x[3, 17] = float("inf")
+    x[4, 18] = float("nan")
+    x[5, 100:] = 0
+    w = torch.linspace(-2, 2, 200)
+    for eps in (1e-5, 0.0):
+        _, _, y = R.rms(x, None, w, eps, torch.float32)
+        got, _, _ = ops.rmsnorm_fwd(x.cuda(), w.cuda(), eps)
+        same(got, y)
+        for fmt in FMTS:
+            q, h = ops.rmsnorm_mx(x.cuda(), w.cuda(), eps, fmt)
+            check_codes(q, y, fmt)
+    big = data((12, 300), torch.bfloat16, 32).cuda()
+    w = torch.ones(128)
+    for a, b in ((big[::2, 16:144], big[1::2, 8:136]), (big[::2, 3:131], big[1::2, 1:129]), (big[:6, :128].t().contiguous().t(), big[6:, :128])):
+        h, _, y = R.rms(a.cpu(), b.cpu(), w, 1e-6, torch.bfloat16)
+        for fmt in FMTS:
+            q, gh = ops.rmsnorm_mx(a, w.cuda(), 1e-6, fmt, residual=b)
+            same(gh, h)
+            check_codes(q, y, fmt)
+    q, h = ops.rmsnorm_mx(big[:0], torch.ones(300, device="cuda"), 1e-6, "mxfp8")
+    assert q.shape == (0, 300)
+
+
+@pytest.mark.parametrize("shape", SHAPES + [(3000, 96), (5000, 33)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", [None, "mxfp8", "mxfp4"])
+def test_rmsnorm_gradients(tops, shape, dtype, fmt):
+    """d: at most ~8 roundings of 32-bit numbers of the size of the terms, and one to the stream's type; dw: a 32-bit sum over up to
+    rows / 256 terms before the rest is added in 64 bits: (rows / 256 + 8) half steps of sum |g xh|"""
+    cols = shape[-1]
+    for residual in (False, True):
+        x, gy, gh = data(shape, dtype, 41), data(shape, dtype, 42, 0.3), data(shape, dtype, 43, 0.3)
+        res = data(shape, dtype, 44) if residual else None
+        w = 1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(3))
+        lx, lw = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        two = [x.reshape(-1, cols), None if res is None else res.reshape(-1, cols)]
+        h, rstd, y = R.rms(*two, w, 1e-6, dtype)
+        inside = torch.ones(h.shape, dtype=torch.bool) if fmt is None else R.fake(y, fmt)[1]
+        rgh = gh.reshape(h.shape) if residual else None
+        d, dw = R.rms_grads(gy.reshape(h.shape), rgh, h, rstd, w, inside)
+        if residual:
+            lr = res.cuda().requires_grad_(True)
+            out, stream = tops.rms_norm(lx, lw, 1e-6, fmt, residual=lr)
+            gx, gr, gw = torch.autograd.grad([out, stream], [lx, lr, lw], [gy.cuda(), gh.cuda()])
+            same(gx, gr)
+        else:
+            out = tops.rms_norm(lx, lw, 1e-6, fmt)
+            gx, gw = torch.autograd.grad(out, [lx, lw], gy.cuda())
+        g, xh = gy.reshape(h.shape).double() * inside, h.double() * rstd
+        size = rstd * ((g * w).abs() + xh.abs() * (g * w * xh).abs().mean(-1, keepdim=True)) + (0 if rgh is None else rgh.double().abs())
+        err = (gx.cpu().reshape(h.shape).double() - d).abs()
+        assert bool((err <= 8 * 2.0 ** -24 * size + HALF[dtype] * d.abs() * 1.001 + 2.0 ** -25 * (dtype == torch.float16) + 1e-44).all()), float(err.max())
+        tol = (h.shape[0] / 256 + 8) * 2.0 ** -24 * (g * xh).abs().sum(0)
+        err = (gw.cpu().double() - dw).abs()
+        assert bool((err <= tol + 1e-44).all()), float((err - tol).max())
+
+
+def test_rmsnorm_gradient_against_differences(tops):
+    """the reference's gradient against central differences of the reference's function in 64 bits, and the kernel's along the same
+    direction"""
+    g = torch.Generator().manual_seed(7)
+    x, w, gy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 70), (70,), (5, 70)))
+    dx, dw = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 70), (70,)))
+
+    def f(t):
+        a = x + t * dx
+        return (gy * a / torch.sqrt((a * a).mean(-1, keepdim=True) + 1e-3) * (w + t * dw)).sum()
+
+    slope = float((f(1e-5) - f(-1e-5)) / 2e-5)
+    lx, lw = x.float().cuda().requires_grad_(True), w.float().cuda().requires_grad_(True)
+    gx, gw = torch.autograd.grad(tops.rms_norm(lx, lw, 1e-3), [lx, lw], gy.float().cuda())
+    mine = float((gx.cpu().double() * dx).sum() + (gw.cpu().double() * dw).sum())
+    # 420 terms of order 1, each a few 32-bit roundings; the difference quotient itself is good to 1e-9
+    assert abs(mine - slope) <= 420 * 16 * 2.0 ** -24, (mine, slope)
+
+
+def test_rmsnorm_gradient_cases(tops):
+    """unused outputs, a weight without gradient, a 16-bit weight, gradients of odd strides, no rows"""
+    x, res, w = data((6, 96), torch.bfloat16, 51).cuda(), data((6, 96), torch.bfloat16, 52).cuda(), data((96,), torch.bfloat16, 53).cuda()
+    a, b, c = x.clone().requires_grad_(True), res.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y, h = tops.rms_norm(a, c, 1e-6, "mxfp8", residual=b)
+    gh = torch.randn_like(h)
+    ga, gb = torch.autograd.grad(h, [a, b], gh, retain_graph=True)
+    same(ga, gh)
+    same(gb, gh)
+    gy = torch.randn(96, 6, device="cuda").to(torch.bfloat16).t()
+    ga, gc = torch.autograd.grad(y, [a, c], gy, retain_graph=True)
+    g2, gc2 = torch.autograd.grad(y, [a, c], gy.contiguous())
+    same(ga, g2)
+    same(gc, gc2)
+    hh, rstd, yy = R.rms(x.cpu(), res.cpu(), w.cpu(), 1e-6, torch.bfloat16)
+    d, dw = R.rms_grads(gy.cpu(), None, hh, rstd, w.cpu(), R.fake(yy, "mxfp8")[1])
+    # one rounding to bf16 on top of the 32-bit arithmetic
+    assert bool(((gc.cpu().double() - dw).abs() <= 2.0 ** -8 * dw.abs() + 1e-5).all())
+    y = tops.rms_norm(a, w, 1e-6)
+    (ga,) = torch.autograd.grad(y, [a], torch.ones_like(y))
+    assert ga.shape == a.shape
+    e = x[:0].clone().requires_grad_(True)
+    c = w.clone().requires_grad_(True)
+    ge, gc = torch.autograd.grad(tops.rms_norm(e, c, 1e-6, "mxfp4"), [e, c], torch.ones(0, 96, device="cuda", dtype=torch.bfloat16))
+    assert ge.shape == (0, 96) and int(torch.count_nonzero(gc)) == 0
+
+
+# ------------------------------------------------------------------------------------------------ product
+def product_case(m, n, k, fmt, seed):
+    a, w = data((m, k), torch.float32, seed), data((n, k), torch.float32, seed + 1, 0.2) * 0.02
+    ca, ba, _ = R.quantize(a, fmt)
+    cw, bw, _ = R.quantize(w, "mxfp4")
+    return (R.pack(ca, fmt), ba, R.values(ca, ba, k, fmt)), (R.pack(cw, "mxfp4"), bw, R.values(cw, bw, k, "mxfp4"))
+
+
+def check_product(got, va, vw, bias, dtype, fmt):
+    """32 bits: sums of at most K / 16 + 16 partial sums, each addition off by at most 2^-23 of sum |a w|.  16 bits: half a step of the
+    result, and for e4m3 what the instruction drops of a product more than 13 places below the largest of its group: measured at a few
+    1e-6 of the result in norm, bounded by 2^-13 of the group's largest product each."""
+    k = va.shape[1]
+    ref = va @ vw.t() + (0 if bias is None else bias.double())
+    size = va.abs() @ vw.abs().t() + (0 if bias is None else bias.double().abs())
+    tol = (k / 16 + 16) * 2.0 ** -23 * size
+    got = got.cpu().double()
+    if dtype != torch.float32:
+        tol = tol + HALF[dtype] * ref.abs() * 1.001 + (2.0 ** -25 if dtype == torch.float16 else 0) + (2.0 ** -13 * size if fmt == "mxfp8" else 0)
+        assert float((got - ref).norm()) <= (HALF[dtype] + 1e-4) * float(ref.norm()) + 1e-6
+    bad = (got - ref).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), float(((got - ref).abs() / (size + 1e-30)).max()))
+
+
+MNK = [(1, 1, 1), (1, 16, 32), (3, 5, 31), (1, 64, 128), (2, 48, 160), (16, 16, 4096), (17, 33, 1000), (33, 100, 96), (48, 256, 512), (64, 64, 640), (65, 130, 2080),
+       (100, 257, 384), (128, 128, 128), (200, 520, 1120), (256, 256, 512), (257, 300, 1024), (333, 1001, 1000), (512, 768, 1056), (600, 264, 4128)]
+
+
+@pytest.mark.parametrize("mnk", MNK)
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product(ops, mnk, fmt):
+    m, n, k = mnk
+    (ca, ba, va), (cw, bw, vw) = product_case(m, n, k, fmt, m + n + k)
+    a, w = ops.MXTensor(ca.cuda(), ba.cuda(), k, fmt), ops.MXTensor(cw.cuda(), bw.cuda(), k, "mxfp4")
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(9))
+    for dtype in DTYPES:
+        check_product(ops.mx_gemm(a, w, dtype=dtype), va, vw, None, dtype, fmt)
+        got = ops.mx_gemm(a, w, bias=bias.cuda(), dtype=dtype)
+        check_product(got, va, vw, bias, dtype, fmt)
+        same(ops.mx_gemm(a, w, bias=bias.cuda(), dtype=dtype), got)      # the same bits again
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_product_wide_scales(ops, fmt, m):
+    """scales of neighbouring blocks far apart, rows of zeros, blocks that stand for NaN: a NaN block makes its own row or column NaN and
+    touches no other"""
+    n, k = 80, 288
+    (ca, ba, va), (cw, bw, vw) = product_case(m, n, k, fmt, 77)
+    g = torch.Generator().manual_seed(8)
+    ba, bw = torch.randint(100, 150, ba.shape, generator=g).to(torch.uint8), torch.randint(100, 150, bw.shape, generator=g).to(torch.uint8)
+    ca[m // 2] = 0
+    one = lambda c, f: c if f == "mxfp8" else torch.stack([c & 15, c >> 4], -1).reshape(c.shape[0], -1)  # noqa: E731
+    va, vw = R.values(one(ca, fmt), ba, k, fmt), R.values(one(cw, "mxfp4"), bw, k, "mxfp4")
+    a, w = ops.MXTensor(ca.cuda(), ba.cuda(), k, fmt), ops.MXTensor(cw.cuda(), bw.cuda(), k, "mxfp4")
+    check_product(ops.mx_gemm(a, w, dtype=torch.float32), va, vw, None, torch.float32, fmt)
+    clean = ops.mx_gemm(a, w, dtype=torch.float32).cpu()
+    ba[m - 1, 4], bw[7, 0] = 255, 255
+    got = ops.mx_gemm(ops.MXTensor(ca.cuda(), ba.cuda(), k, fmt), ops.MXTensor(cw.cuda(), bw.cuda(), k, "mxfp4"), dtype=torch.float32).cpu()
+    assert bool(torch.isnan(got[m - 1]).all()) and bool(torch.isnan(got[:, 7]).all())
+    keep = torch.ones(m, n, dtype=torch.bool)
+    keep[m - 1], keep[:, 7] = False, False
+    assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [3, 150])
+def test_product_reads_and_writes_only_its_own(ops, fmt, m):
+    """operands cut out of larger tensors whose other bytes stand for NaN; leading dimensions; no rows, no columns"""
+    n, k = 70, 224
+    (ca, ba, va), (cw, bw, vw) = product_case(m, n, k, fmt, 5)
+
+    def inside(c, s):
+        big = torch.full((c.shape[0] + 2, c.shape[1] + 48), 0x7F, dtype=torch.uint8, device="cuda")
+        big[1:-1, 16:16 + c.shape[1]] = c.cuda()
+        sc = torch.full((s.shape[0] + 2, s.shape[1] + 3), 255, dtype=torch.uint8, device="cuda")
+        sc[1:-1, 1:1 + s.shape[1]] = s.cuda()
+        return big[1:-1, 16:16 + c.shape[1]], sc[1:-1, 1:1 + s.shape[1]]
+
+    a, w = ops.MXTensor(*inside(ca, ba), k, fmt), ops.MXTensor(*inside(cw, bw), k, "mxfp4")
+    got = ops.mx_gemm(a, w, dtype=torch.float32)
+    check_product(got, va, vw, None, torch.float32, fmt)
+    dense = ops.MXTensor(ca.cuda().reshape(1, m, -1), ba.cuda().reshape(1, m, -1), k, fmt)
+    same(ops.mx_gemm(dense, w, dtype=torch.float32), got.unsqueeze(0))
+    assert ops.mx_gemm(ops.MXTensor(a.codes[:0], a.scales[:0], k, fmt), w).shape == (0, n)
+    assert ops.mx_gemm(a, ops.MXTensor(w.codes[:0], w.scales[:0], k, "mxfp4")).shape == (m, 0)
+    # the output's neighbours in memory stay as they were (C entry with a row pitch of its own)
+    from edadm import lib
+    out = torch.full((m + 2, n + 5), 7.0, device="cuda")
+    c, ldc, s, lds, _ = a._rows()
+    d, ldd, t, ldt, _ = w._rows()
+    lib.call("edadm_mx_gemm", c.data_ptr(), ldc, s.data_ptr(), lds, 4 if fmt == "mxfp4" else 8, d.data_ptr(), ldd, t.data_ptr(), ldt, m, n, k, None,
+             out[1:, 2:].data_ptr(), n + 5, 0, torch.cuda.current_stream().cuda_stream)
+    same(out[1:-1, 2:2 + n], got)
+    out[1:-1, 2:2 + n] = 7.0
+    assert bool((out == 7.0).all())
+
+
+# ------------------------------------------------------------------------------------------------ together
+def block_chain(ops, x, res, nw, w1, w2, fmt):
+    q, h = ops.rmsnorm_mx(x, nw, 1e-6, fmt, residual=res)
+    u = ops.mx_gemm(q, w1, dtype=torch.bfloat16)
+    y = ops.mx_gemm(ops.mx_quantize(u, fmt), w2, dtype=torch.bfloat16)
+    return h, u, y
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [1, 37, 320])
+def test_a_feed_forward_run(ops, fmt, rows):
+    """norm -> product -> quantise -> product, as a quantised feed-forward block runs them, against the 64-bit reference fed step by step
+    with the run's own intermediate tensors; on a side stream, and captured into two graphs that are replayed in turn on new inputs with
+    eager work between them"""
+    C, D = 320, 1280
+    nw = (1 + 0.1 * torch.randn(C, generator=torch.Generator().manual_seed(1))).cuda()
+    w1 = ops.mx_quantize((data((D, C), torch.float32, 61, 0.1) * 0.05).cuda(), "mxfp4")
+    w2 = ops.mx_quantize((data((C, D), torch.float32, 62, 0.1) * 0.05).cuda(), "mxfp4")
+    v1, v2 = ops.mx_dequantize(w1).cpu().double(), ops.mx_dequantize(w2).cpu().double()
+    inputs = [(data((rows, C), torch.bfloat16, 70 + i).cuda(), data((rows, C), torch.bfloat16, 80 + i).cuda()) for i in range(4)]
+    want = [block_chain(ops, x, r, nw, w1, w2, fmt) for x, r in inputs]
+    x, r = inputs[0]
+    h, _, y = R.rms(x.cpu(), r.cpu(), nw.cpu(), 1e-6, torch.bfloat16)
+    same(want[0][0], h)
+    check_product(want[0][1], R.fake(y, fmt)[0], v1, None, torch.bfloat16, fmt)
+    check_product(want[0][2], R.fake(want[0][1].cpu(), fmt)[0], v2, None, torch.bfloat16, fmt)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = block_chain(ops, *inputs[1], nw, w1, w2, fmt)
+    torch.cuda.current_stream().wait_stream(side)
+    for g, e in zip(got, want[1]):
+        same(g, e)
+    graphs = []
+    for _ in range(2):
+        sx, sr = torch.zeros_like(x), torch.zeros_like(r)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block_chain(ops, sx, sr, nw, w1, w2, fmt)
+        graphs.append((graph, sx, sr, out))
+    for i in (2, 3, 0, 1, 2):
+        for k, (graph, sx, sr, out) in enumerate(graphs):
+            j = (i + k) % 4
+            sx.copy_(inputs[j][0])
+            sr.copy_(inputs[j][1])
+            graph.replay()
+            junk = torch.randn(1 << 16, device="cuda").sum()
+            torch.cuda.synchronize()
+            for g, e in zip(out, want[j]):
+                same(g, e)
+            del junk
+
+
+def test_a_calibration_step(ops, tops):
+    """the training form of the same block: norm with fake-quantised output, fake-quantised weight, the framework's own differentiable
+    product; gradients of every leaf against the 64-bit formulas"""
+    from edadm import contract
+    rows, C, D = 48, 96, 64
+    x, res, w = data((rows, C), torch.float32, 91, 0.3), data((rows, C), torch.float32, 92, 0.3), data((D, C), torch.float32, 93, 0.2) * 0.1
+    nw = 1 + 0.1 * torch.randn(C, generator=torch.Generator().manual_seed(4))
+    gy, gh = data((rows, D), torch.float32, 94, 0.1), data((rows, C), torch.float32, 95, 0.1)
+    lx, lr, lw, ln = (t.cuda().requires_grad_(True) for t in (x, res, w, nw))
+    y, h = tops.rms_norm(lx, ln, 1e-6, "mxfp8", residual=lr)
+    out = contract.linear(y, tops.mx_fake_quant(lw, "mxfp4"))
+    got = torch.autograd.grad([out, h], [lx, lr, ln, lw], [gy.cuda(), gh.cuda()])
+    rh, rstd, ry = R.rms(x, res, nw, 1e-6, torch.float32)
+    fy, iy = R.fake(ry, "mxfp8")
+    fw, iw = R.fake(w, "mxfp4")
+    d, dn = R.rms_grads(gy.double() @ fw, gh, rh, rstd, nw, iy)
+    dw = (gy.double().t() @ fy) * iw
+    # the products of the calibration graph are good to 2e-5 of their range (their own tests); everything after them to 1e-6
+    for g, e in zip(got, (d, d, dn, dw)):
+        assert float((g.cpu().double() - e).abs().max()) <= 5e-5 * float(e.abs().max())
+    check = float((out.detach().cpu().double() - fy @ fw.t()).abs().max())
+    assert check <= 2e-5 * float((fy @ fw.t()).abs().max())
+
+
+def test_training_step_in_a_graph(tops):
+    """forward and backward of the norm captured together (static leaves, gradients read out of the graph's own tensors), replayed on
+    changed inputs"""
+    x, w = torch.zeros(130, 160, device="cuda"), torch.ones(160, device="cuda")
+    gy = torch.zeros(130, 160, device="cuda")
+
+    def step():
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = tops.rms_norm(a, b, 1e-6, "mxfp4")
+        return (y.detach(),) + torch.autograd.grad(y, [a, b], gy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        x.copy_(data((130, 160), torch.float32, 200 + i))
+        gy.copy_(data((130, 160), torch.float32, 300 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for g, e in zip(got, step()):
+            same(g, e)

@@ -1,0 +1,107 @@
+"""CPU: what the microscaled operators refuse (nothing is launched), and the reference the GPU tests use against the formats' own tables."""
+import pytest
+import torch
+
+import mx_reference as R
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from edadm import ops as _ops
+    return _ops
+
+
+def test_reference_formats():
+    assert R.E4M3[-1] == 448 and R.E4M3[1] == 2.0 ** -9 and len(R.E4M3) == 127
+    codes = torch.arange(0, 127, dtype=torch.uint8)
+    assert torch.equal(codes.view(torch.float8_e4m3fn).double(), R.E4M3)
+    x = torch.linspace(-500, 500, 4096).reshape(1, -1)
+    v = x.double().clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    v = v & 127
+    assert torch.equal(R.nearest(x.double().abs(), "mxfp8").to(torch.uint8), v)
+    # ties of e2m1 go to the even code
+    t = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0], dtype=torch.float64)
+    assert R.E2M1[R.nearest(t, "mxfp4")].tolist() == [0, 1, 1, 2, 2, 4, 4, 6]
+    code, byte, inside = R.quantize(torch.tensor([[0.0] * 32 + [8.0, 7.9] + [0.1] * 30 + [7.9]]), "mxfp4")
+    assert byte.tolist() == [[0, 128, 127]] and inside[0].tolist() == [True] * 64 + [False]
+
+
+def test_refusals_on_the_host(ops):
+    from edadm import lib, train_ops
+    E = lib.EdadmError
+    x, w = torch.zeros(4, 64), torch.ones(64)
+    for call in (lambda: ops.mx_quantize(x, "mxfp8"), lambda: ops.mx_fake_quant_fwd(x, "mxfp4"), lambda: ops.rmsnorm_mx(x, w, 1e-6, "mxfp8"),
+                 lambda: train_ops.mx_fake_quant(x, "mxfp4"), lambda: train_ops.rms_norm(x, w, 1e-6)):
+        with pytest.raises(E, match="device"):
+            call()
+    for fmt in ("mxfp6", "int8", None, 4):
+        with pytest.raises(E, match="format"):
+            ops.mx_quantize(x, fmt)
+    with pytest.raises(E, match="format"):
+        ops.rmsnorm_mx(x, w, 1e-6, None)
+    with pytest.raises(E, match="float32"):
+        ops.mx_quantize(x.double(), "mxfp4")
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    q = ops.MXTensor(codes, scales, 64, "mxfp4")
+    assert q.shape == (4, 64)
+    with pytest.raises(E, match="device"):
+        ops.mx_dequantize(q)
+    with pytest.raises(E, match="device"):
+        ops.mx_gemm(q, q)
+    for args in ((codes, scales, 65, "mxfp4"), (codes, scales, 64, "mxfp8"), (codes.to(torch.int8), scales, 64, "mxfp4"), (codes[:3], scales, 64, "mxfp4"),
+                 (codes, scales[:, :1], 64, "mxfp4"), (codes, scales, 0, "mxfp4"), (codes, scales, 64, "fp4")):
+        with pytest.raises(E):
+            ops.MXTensor(*args)
+    e = ops.MXTensor(torch.zeros(4, 64, dtype=torch.uint8), scales, 64, "mxfp8")
+    with pytest.raises(E, match="second operand"):
+        ops.mx_gemm(q, e)
+    with pytest.raises(E, match="elements a row"):
+        ops.mx_gemm(q, ops.MXTensor(codes[:, :16], scales[:, :1], 32, "mxfp4"))
+    with pytest.raises(E, match="bias"):
+        ops.mx_gemm(q, q, bias=torch.zeros(5))
+    with pytest.raises(E, match="bias"):
+        ops.mx_gemm(q, q, bias=torch.zeros(4, dtype=torch.bfloat16))
+    with pytest.raises(E, match="float32"):
+        ops.mx_gemm(q, q, dtype=torch.float64)
+    with pytest.raises(E, match="MXTensor"):
+        ops.mx_gemm(x, q)
+
+
+def test_entry_points_refuse_bad_arguments():
+    """status -22 before anything is launched: null pointers, types, formats and pitches that do not fit"""
+    from edadm import lib
+    l = lib.load()
+    p = 1 << 20                                                  # an aligned address that is never read
+    assert l.edadm_mx_quantize(None, 64, 0, p, 32, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 63, 0, p, 32, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 3, p, 32, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 32, p, 2, 4, 64, 6, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 16, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p + 8, 32, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 40, p, 2, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 32, p, 1, 4, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 32, p, 2, -1, 64, 4, None) == -22
+    assert l.edadm_mx_quantize(p, 64, 0, p, 32, p, 2, 4, 0, 4, None) == -22
+    assert l.edadm_mx_quantize(None, 64, 0, None, 32, None, 2, 0, 64, 4, None) == 0          # no rows: nothing to do
+    assert l.edadm_mx_dequantize(p, 32, p, 2, 4, None, 64, 0, 4, 64, None) == -22
+    assert l.edadm_mx_dequantize(p, 32, p, 2, 8, p, 64, 0, 4, 64, None) == -22
+    assert l.edadm_mx_fake_quant_fwd(p, 64, 0, p, 63, 4, 64, 4, None) == -22
+    assert l.edadm_mx_fake_quant_bwd(None, 64, p, 64, 0, p, 64, 4, 64, 4, None) == -22
+    n = l.edadm_rmsnorm_max_cols()
+    assert n >= 16384
+    assert l.edadm_rmsnorm_fwd(p, n + 1, None, 0, 0, p, 1, None, 0, None, p, n + 1, None, 0, 1, n + 1, 1e-6, 0, 0, None) == -22
+    assert l.edadm_rmsnorm_fwd(p, 64, p, 64, 0, p, 1, None, 0, None, p, 64, None, 0, 1, 64, 1e-6, 0, 0, None) == -22
+    assert l.edadm_rmsnorm_fwd(p, 64, None, 0, 0, p, 1, None, 0, None, p, 64, None, 0, 1, 64, -1.0, 0, 0, None) == -22
+    assert l.edadm_rmsnorm_fwd(p, 64, None, 0, 0, p, 1, None, 0, None, p, 64, None, 2, 1, 64, 1e-6, 8, 0, None) == -22
+    assert l.edadm_rmsnorm_bwd(p, 64, None, 0, p, 64, 0, p, p, 1, p, 64, p, None, 1, 64, 0, None) == -22
+    assert l.edadm_rmsnorm_bwd(p, 64, None, 0, p, 64, 0, None, p, 1, p, 64, None, None, 1, 64, 0, None) == -22
+    assert l.edadm_rmsnorm_bwd_ws_floats(0, 64) == 0 and l.edadm_rmsnorm_bwd_ws_floats(5, 40) >= 5 * 40
+    g = l.edadm_mx_gemm
+    assert g(p, 32, p, 2, 4, p, 32, p, 2, 0, 8, 64, None, None, 8, 0, None) == 0
+    assert g(p, 32, p, 2, 4, p, 32, p, 2, 4, 8, 64, None, None, 8, 0, None) == -22
+    assert g(p, 32, p, 2, 4, p, 32, p, 2, 4, 8, 64, None, p, 7, 0, None) == -22
+    assert g(p, 32, p, 2, 8, p, 32, p, 2, 4, 8, 64, None, p, 8, 0, None) == -22
+    assert g(p, 32, p, 1, 4, p, 32, p, 2, 4, 8, 64, None, p, 8, 0, None) == -22
+    assert g(p, 32, p, 2, 4, p, 24, p, 2, 4, 8, 64, None, p, 8, 0, None) == -22
+    assert g(p, 32, p, 2, 4, p, 32, p, 2, 4, 8, 64, None, p, 8, 3, None) == -22
+    assert g(p, 32, p, 2, 4, p, 32, p, 2, 4, 8, 0, None, p, 8, 0, None) == -22
