@@ -26,6 +26,13 @@ struct MxArgs {
     int nblk;                          // blocks of 32 along K
 };
 
+template <int V> struct mx_int { static constexpr int value = V; };
+template <int N, typename F> __device__ __forceinline__ void mx_unroll(F&& f) {
+    if constexpr (N > 0) {
+        mx_unroll<N - 1>(f);
+        f(mx_int<N - 1>{});
+    }
+}
 __device__ __forceinline__ mx_i8 frag4(uint4 a) { return mx_i8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}; }
 __device__ __forceinline__ mx_i8 frag8(uint4 a, uint4 b) { return mx_i8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w}; }
 
@@ -72,7 +79,9 @@ template <int ODT> __device__ __forceinline__ void mx_out4(const MxArgs& a, int6
             else { p[0] = (uint16_t)x; p[1] = (uint16_t)(x >> 16); p[2] = (uint16_t)y; p[3] = (uint16_t)(y >> 16); }
         }
     } else {
-        for (int i = 0; i < 4 && n + i < a.N; ++i) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (n + i >= a.N) break;
             const float s = a.bias ? v[i] + a.bias[n + i] : v[i];
             if constexpr (ODT == MX_F32) ((float*)a.out)[m * a.ldo + n + i] = s;
             else ((uint16_t*)a.out)[m * a.ldo + n + i] = (uint16_t)mx_pair<ODT>(s, 0.f);
@@ -154,6 +163,224 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxArgs a, int strips) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ many rows
+// A workgroup of WM x WN waves owns a BM x BN tile, a wave MT x NT instructions of 32 x 32 x 64 of it.  K advances by a step of 128
+// (8-bit a) or 256 (4-bit a) elements: 128 bytes of every row of a, 64 or 128 of w.  A ring of steps' operands lies in LDS; they arrive by
+// direct-to-LDS loads, 16 bytes a lane, and are read in whole fragments, each while the one before it multiplies.
+//
+// Hand-off: one barrier a step, in front of its last sub-step.  Behind it the next step's operands are complete for every wave, so that
+// their first fragments are fetched while the last sub-step multiplies, and the load of the step after next goes out, a full step
+// ahead of its use.  8-bit a: three slots of 48 KB; that load fills the slot of the step before, which no wave reads any more, and a
+// fragment of a is fetched over the one just used (two sets of them and the sums would not fit 256 registers).  4-bit a: two slots of
+// 64 KB; the load fills this step's slot, so its last fragments are awaited in front of the barrier, and there are two sets.
+//
+// LDS order: 16-byte piece p of row r lies at piece p ^ ((r >> 1) & 7) (rows of 128 bytes) or p ^ ((r >> 2) & 3) (rows of 64), so that
+// the 16 lanes of a quarter of a fragment read hit 16 different 16-byte groups of banks; the loads permute their source addresses.
+//
+// Scales stay in registers: a lane holds the four (eight) bytes of its row for a step, shifted by its half of the wave, so that the
+// instruction's byte selector walks the sub-steps.  What is left of K behind the whole steps is fetched straight into registers.
+typedef float mx_f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
+
+// 16 bytes a lane from a wave-uniform base plus a per-lane offset into LDS at a wave-uniform address (lane order); not tracked by the
+// compiler, so that fragment reads of the other buffer do not wait for it: the kernel waits for all of them in front of its barrier
+__device__ __forceinline__ void mx_dma16(const void* base, uint32_t voff, uint32_t lds) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(base), "s"(lds)
+                 : "memory");
+}
+
+// a wave-uniform address in scalar registers
+__device__ __forceinline__ const void* mx_uniform(const void* p) {
+    const uint64_t u = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+    return (const void*)((uint64_t)hi << 32 | lo);
+}
+
+template <int AF, bool EXACT, int T>
+__device__ __forceinline__ mx_f16v mx_mma32(mx_i8 w, mx_i8 a, mx_f16v c, uint32_t sw, uint32_t sa) {
+    constexpr int B = (T & 1) * 2;                                    // the sub-step's byte of the lane's scales
+    if constexpr (AF == MX_FP4) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 4, 4, B, (int)sw, B, (int)sa);
+    else if constexpr (!EXACT) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, c, 4, 0, B, (int)sw, B, (int)sa);
+    else {
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, part_lo(a), c, 4, 0, B, (int)sw, B, (int)sa);
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, part_hi(a), c, 4, 0, B, (int)sw, B, (int)sa);
+    }
+}
+
+template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT>
+__global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int tn) {
+    constexpr int THREADS = 64 * WM * WN, BM = 32 * WM * MT, BN = 32 * WN * NT;
+    constexpr int STEP = AF == MX_FP4 ? 8 : 4;                        // blocks of 32 a step
+    constexpr int SUB = STEP / 2;                                     // sub-steps of 64
+    constexpr int WROW = AF == MX_FP4 ? 128 : 64;                     // bytes of a row of w a step
+    constexpr int ABYTES = BM * 128, WBYTES = BN * WROW, STAGE = ABYTES + WBYTES;
+    constexpr int RING = AF == MX_FP4 ? 2 : 3;                        // steps' operands in LDS
+    constexpr int AI = ABYTES / (THREADS * 16), WI = WBYTES / (THREADS * 16);   // load instructions a wave
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wm = wave / WN, wn = wave % WN;
+
+    // tile of this workgroup: workgroups go round the 8 XCDs, so every XCD gets a run of neighbouring tiles, walked eight tile rows
+    // at a time down the rows first: the tiles an XCD works on together share rows of a and of w in its L2
+    const int total = tm * tn, each = total / 8, more = total % 8, x = (int)(blockIdx.x & 7);
+    const int t = (x < more ? x * (each + 1) : more * (each + 1) + (x - more) * each) + (int)(blockIdx.x >> 3);
+    const int band = t / (8 * tn), in = t - band * 8 * tn, high = min(8, tm - band * 8);
+    const int64_t m0 = (int64_t)(band * 8 + in % high) * BM, n0 = (int64_t)(in / high) * BN;
+
+    const uint8_t* ab = a.A + m0 * a.lda;
+    const uint8_t* wb = a.W + n0 * a.ldw;
+    uint32_t av[AI], wv[WI];
+#pragma unroll
+    for (int i = 0; i < AI; ++i) {
+        const int row = (i * THREADS + (int)threadIdx.x) >> 3, p = (lane & 7) ^ ((row >> 1) & 7);
+        av[i] = (uint32_t)min((int64_t)row, a.M - 1 - m0) * (uint32_t)a.lda + p * 16;       // past the last row: read that one
+    }
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+        const int per = WROW / 16, row = (i * THREADS + (int)threadIdx.x) / per;
+        const int p = (lane % per) ^ (WROW == 128 ? (row >> 1) & 7 : (row >> 2) & 3);
+        wv[i] = (uint32_t)min((int64_t)row, a.N - 1 - n0) * (uint32_t)a.ldw + p * 16;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    auto load = [&](int at) {
+        const void *ua = mx_uniform(ab), *uw = mx_uniform(wb);
+        const uint32_t la = lds0 + at + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < AI; ++i) mx_dma16(ua, av[i], __builtin_amdgcn_readfirstlane(la + i * (THREADS * 16)));
+#pragma unroll
+        for (int i = 0; i < WI; ++i) mx_dma16(uw, wv[i], __builtin_amdgcn_readfirstlane(la + ABYTES + i * (THREADS * 16)));
+        ab += 128;
+        wb += WROW;
+    };
+    // scale rows as 32-bit offsets from the tile's first
+    const uint8_t *asb = a.As + m0 * a.ldas, *wsb = a.Ws + n0 * a.ldws;
+    uint32_t aso[MT], wso[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) aso[i] = (uint32_t)min((int64_t)((wm * MT + i) * 32 + r), a.M - 1 - m0) * (uint32_t)a.ldas;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wso[j] = (uint32_t)min((int64_t)((wn * NT + j) * 32 + r), a.N - 1 - n0) * (uint32_t)a.ldws;
+    constexpr int SD = STEP / 4;                                      // dwords of scales a row and step
+    uint32_t sa[MT][SD], sw[NT][SD], sa2[MT][SD], sw2[NT][SD];
+    auto scales = [&](int step) {
+#pragma unroll
+        for (int d = 0; d < SD; ++d) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sa2[i][d] = *(const mx_u32*)(asb + step * STEP + 4 * d + aso[i]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) sw2[j][d] = *(const mx_u32*)(wsb + step * STEP + 4 * d + wso[j]);
+        }
+    };
+    auto take = [&]() {
+#pragma unroll
+        for (int d = 0; d < SD; ++d) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sa[i][d] = sa2[i][d] >> (8 * q);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) sw[j][d] = sw2[j][d] >> (8 * q);
+        }
+    };
+    // fragment i of a (j of w) of sub-step t in ring slot `at` (bytes): the swizzle depends on the lane alone, so that all rows of a
+    // sub-step share one address
+    const int sz = (r >> 1) & 7, szw = WROW == 128 ? sz : (r >> 2) & 3;
+    const uint8_t *pa = smem + (wm * MT * 32 + r) * 128, *pw = smem + ABYTES + (wn * NT * 32 + r) * WROW;
+    auto fragx = [&](int at, int t, int i) {
+        if constexpr (AF == MX_FP4) return frag4(*(const uint4*)(pa + at + ((2 * t + q) ^ sz) * 16 + i * 4096));
+        else return frag8(*(const uint4*)(pa + at + ((4 * t + q) ^ sz) * 16 + i * 4096), *(const uint4*)(pa + at + ((4 * t + 2 + q) ^ sz) * 16 + i * 4096));
+    };
+    auto fragw = [&](int at, int t, int j) { return frag4(*(const uint4*)(pw + at + ((2 * t + q) ^ szw) * 16 + j * 32 * WROW)); };
+
+    mx_f16v acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    const int steps = a.nblk / STEP;
+    if (steps) {
+        mx_i8 fx[2][MT], fw[2][NT];
+        load(0);
+        if (RING == 3 && steps > 1) load(STAGE);
+        scales(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        take();
+        if (steps > 1) scales(1);
+        if (RING == 2 && steps > 1) load(STAGE);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fx[0][i] = fragx(0, 0, i);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
+        int at = 0, next = steps > 1 ? STAGE : 0, fill = RING == 3 ? 2 * STAGE : 0;
+        for (int s = 0; s < steps; ++s) {
+            mx_unroll<SUB>([&](auto tt) {
+                constexpr int t = decltype(tt)::value, nt = (t + 1) % SUB, fb = t & 1;
+                if constexpr (t == SUB - 1) {
+                    if constexpr (RING == 2) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    if (s + 2 < steps) load(fill);
+                }
+                // behind the last step the next slot's old contents are fetched and not used
+                const int from = t == SUB - 1 ? next : at;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) fw[fb ^ 1][j] = fragw(from, nt, j);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fx[fb ^ 1][i] = fragx(from, nt, i);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sw[j][t / 2], sa[i][t / 2]);
+            });
+            if (s + 1 < steps) {
+                take();
+                if (s + 2 < steps) scales(s + 2);
+            }
+            if constexpr (RING == 2) { const int keep = at; at = next; next = keep; fill = at; }
+            else { const int keep = at; at = next; next = fill; fill = keep; }
+        }
+    }
+    for (int b = steps * STEP; b < a.nblk; b += 2) {                  // the rest of K, two blocks at a time
+        const bool in = b + q < a.nblk;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        mx_i8 fx[MT], fw[NT];
+        uint32_t ra[MT], rw[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int64_t row = min(m0 + (wm * MT + i) * 32 + r, a.M - 1);
+            const uint8_t* p = a.A + row * a.lda;
+            if constexpr (AF == MX_FP4) fx[i] = frag4(in ? *(const uint4*)(p + (int64_t)(b + q) * 16) : zero);
+            else fx[i] = frag8(*(const uint4*)(p + (int64_t)b * 32 + q * 16), b + 1 < a.nblk ? *(const uint4*)(p + (int64_t)b * 32 + 32 + q * 16) : zero);
+            ra[i] = in ? asb[aso[i] + b + q] : 127u;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int64_t row = min(n0 + (wn * NT + j) * 32 + r, a.N - 1);
+            fw[j] = frag4(in ? *(const uint4*)(a.W + row * a.ldw + (int64_t)(b + q) * 16) : zero);
+            rw[j] = in ? wsb[wso[j] + b + q] : 127u;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], rw[j], ra[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const mx_f4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                mx_out4<ODT>(a, m0 + (wm * MT + i) * 32 + r, n0 + (wn * NT + j) * 32 + 8 * g + 4 * q, v);
+            }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 template <int AF, bool EXACT, int ODT> static int launch_rows(const MxArgs& a, hipStream_t st) {
     const int64_t mt = (a.M + 15) / 16;
@@ -168,7 +395,35 @@ template <int AF, bool EXACT, int ODT> static int launch_rows(const MxArgs& a, h
     return edadm_launch_status();
 }
 
-template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hipStream_t st) { return launch_rows<AF, EXACT, ODT>(a, st); }
+template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static int launch_tile(const MxArgs& a, hipStream_t st) {
+    constexpr int BM = 32 * WM * MT, BN = 32 * WN * NT;
+    constexpr int LDS = (AF == MX_FP4 ? 2 : 3) * (BM * 128 + BN * (AF == MX_FP4 ? 128 : 64));
+    const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+    if (tm > 0x7fffffff / 8 || tn > 0x7fffffff / 8 || tm * tn > 0x7fffffff / 8) return EDADM_EINVAL;
+    auto* k = &k_mx_tile<AF, WM, WN, MT, NT, EXACT, ODT>;
+    if (LDS > 65536) {
+        // once per kernel and device; setting it again is harmless
+        static bool done[EDADM_MAX_DEVICES] = {};
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= EDADM_MAX_DEVICES) return EDADM_EIO;
+        if (!done[dev]) {
+            if (hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return EDADM_EIO;
+            done[dev] = true;
+        }
+    }
+    k<<<(unsigned)(tm * tn), 64 * WM * WN, LDS, st>>>(a, (int)tm, (int)tn);
+    return edadm_launch_status();
+}
+
+template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hipStream_t st) {
+    // the tiled kernel's 32-bit row offsets: 256 rows of a and of w under 4 GB
+    const bool fits = a.lda < (1 << 23) && a.ldw < (1 << 23) && a.ldas < (1 << 23) && a.ldws < (1 << 23);
+    if (a.M <= 64 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
+    const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256), mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+    if (big >= 200) return launch_tile<AF, 2, 2, 4, 4, EXACT, ODT>(a, st);
+    if (mid >= 200) return launch_tile<AF, 2, 2, 2, 2, EXACT, ODT>(a, st);
+    return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
+}
 
 static inline bool mx_side_ok(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int64_t rows, int64_t nb, int fmt) {
     return c && s && (uintptr_t)c % 16 == 0 && ld >= nb * (fmt == MX_FP4 ? 16 : 32) && (rows <= 1 || ld % 16 == 0) && lds >= nb;
