@@ -229,7 +229,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     const int total = tm * tn, each = total / 8, more = total % 8, x = (int)(blockIdx.x & 7);
     const int t = (x < more ? x * (each + 1) : more * (each + 1) + (x - more) * each) + (int)(blockIdx.x >> 3);
     const int band = t / (8 * tn), in = t - band * 8 * tn, high = min(8, tm - band * 8);
-    const int64_t m0 = (int64_t)(band * 8 + in % high) * BM, n0 = (int64_t)(in / high) * BN;
+    // divided by the vector unit, uniform all the same
+    const int ti = __builtin_amdgcn_readfirstlane(band * 8 + in % high), tj = __builtin_amdgcn_readfirstlane(in / high);
+    const int64_t m0 = (int64_t)ti * BM, n0 = (int64_t)tj * BN;
 
     const uint8_t* ab = a.A + m0 * a.lda;
     const uint8_t* wb = a.W + n0 * a.ldw;
@@ -246,15 +248,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         wv[i] = (uint32_t)min((int64_t)row, a.N - 1 - n0) * (uint32_t)a.ldw + p * 16;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    auto load = [&](int at) {
-        const void *ua = mx_uniform(ab), *uw = mx_uniform(wb);
+    // one load instruction (of AI + WI) of the step at `ab`, `wb`
+    auto load1 = [&](int at, int i) {
         const uint32_t la = lds0 + at + wave * 1024;
-#pragma unroll
-        for (int i = 0; i < AI; ++i) mx_dma16(ua, av[i], __builtin_amdgcn_readfirstlane(la + i * (THREADS * 16)));
-#pragma unroll
-        for (int i = 0; i < WI; ++i) mx_dma16(uw, wv[i], __builtin_amdgcn_readfirstlane(la + ABYTES + i * (THREADS * 16)));
+        if (i < AI) mx_dma16(mx_uniform(ab), av[i < AI ? i : 0], __builtin_amdgcn_readfirstlane(la + i * (THREADS * 16)));
+        else mx_dma16(mx_uniform(wb), wv[i < AI ? 0 : i - AI], __builtin_amdgcn_readfirstlane(la + ABYTES + (i - AI) * (THREADS * 16)));
+    };
+    auto advance = [&]() {
         ab += 128;
         wb += WROW;
+    };
+    auto load = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < AI + WI; ++i) load1(at, i);
+        advance();
     };
     // scale rows as 32-bit offsets from the tile's first
     const uint8_t *asb = a.As + m0 * a.ldas, *wsb = a.Ws + n0 * a.ldws;
@@ -264,23 +271,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
     for (int j = 0; j < NT; ++j) wso[j] = (uint32_t)min((int64_t)((wn * NT + j) * 32 + r), a.N - 1 - n0) * (uint32_t)a.ldws;
     constexpr int SD = STEP / 4;                                      // dwords of scales a row and step
-    uint32_t sa[MT][SD], sw[NT][SD], sa2[MT][SD], sw2[NT][SD];
+    // raw: as loaded, two steps ahead;  nx: shifted, the next step's;  sa, sw: this step's
+    uint32_t ra[MT][SD], rw[NT][SD], na[MT][SD], nw[NT][SD], sa[MT][SD], sw[NT][SD];
     auto scales = [&](int step) {
+        const uint8_t *ua = asb + step * STEP, *uw = wsb + step * STEP;
 #pragma unroll
         for (int d = 0; d < SD; ++d) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) sa2[i][d] = *(const mx_u32*)(asb + step * STEP + 4 * d + aso[i]);
+            for (int i = 0; i < MT; ++i) ra[i][d] = *(const mx_u32*)(ua + aso[i] + 4 * d);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) sw2[j][d] = *(const mx_u32*)(wsb + step * STEP + 4 * d + wso[j]);
+            for (int j = 0; j < NT; ++j) rw[j][d] = *(const mx_u32*)(uw + wso[j] + 4 * d);
+        }
+    };
+    // pinned where it stands: moved down, it would wait for loads issued after those it needs
+    auto shift = [&]() {
+#pragma unroll
+        for (int d = 0; d < SD; ++d) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) { na[i][d] = ra[i][d] >> (8 * q); asm volatile("" : "+v"(na[i][d])); }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) { nw[j][d] = rw[j][d] >> (8 * q); asm volatile("" : "+v"(nw[j][d])); }
         }
     };
     auto take = [&]() {
 #pragma unroll
         for (int d = 0; d < SD; ++d) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) sa[i][d] = sa2[i][d] >> (8 * q);
+            for (int i = 0; i < MT; ++i) sa[i][d] = na[i][d];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) sw[j][d] = sw2[j][d] >> (8 * q);
+            for (int j = 0; j < NT; ++j) sw[j][d] = nw[j][d];
         }
     };
     // fragment i of a (j of w) of sub-step t in ring slot `at` (bytes): the swizzle depends on the lane alone, so that all rows of a
@@ -309,6 +328,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         scales(0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
+        shift();
         take();
         if (steps > 1) scales(1);
         if (RING == 2 && steps > 1) load(STAGE);
@@ -316,59 +336,82 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         for (int i = 0; i < MT; ++i) fx[0][i] = fragx(0, 0, i);
 #pragma unroll
         for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
-        int at = 0, next = steps > 1 ? STAGE : 0, fill = RING == 3 ? 2 * STAGE : 0;
-        for (int s = 0; s < steps; ++s) {
+        int at = 0, next = STAGE, fill = RING == 3 ? 2 * STAGE : 0;
+        // one step; MORE steps behind it (0, 1 or at least 2) decide what is fetched.  No branch inside: the compiler would move a
+        // sub-step's multiplications behind it, away from the fetches they hide
+        auto step = [&](int s, auto more) {
+            constexpr int MORE = decltype(more)::value;
             mx_unroll<SUB>([&](auto tt) {
                 constexpr int t = decltype(tt)::value, nt = (t + 1) % SUB, fb = t & 1;
-                if constexpr (t == SUB - 1) {
+                constexpr bool LAST = t == SUB - 1;
+                if constexpr (LAST && MORE > 0) {
                     if constexpr (RING == 2) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    if (s + 2 < steps) load(fill);
+                    // the wait above covered the next step's scales too: they leave their registers here, in front of any new load
+                    shift();
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (MORE > 1) scales(s + 2);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                // behind the last step the next slot's old contents are fetched and not used
-                const int from = t == SUB - 1 ? next : at;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) fw[fb ^ 1][j] = fragw(from, nt, j);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) fx[fb ^ 1][i] = fragx(from, nt, i);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sw[j][t / 2], sa[i][t / 2]);
+                // behind each multiplication one fragment is fetched for the next sub-step and, behind the barrier, one load goes out
+                const int from = LAST ? next : at;
+                constexpr bool FETCH = !LAST || MORE > 0, LOAD = LAST && MORE > 1;
+                constexpr int OPS = MT * NT, READS = MT + NT, LOADS = AI + WI;
+                mx_unroll<OPS>([&](auto kk) {
+                    constexpr int k = decltype(kk)::value, i = k / NT, j = k % NT;
+                    acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sw[j][t / 2], sa[i][t / 2]);
+                    if constexpr (FETCH) {
+                        constexpr int r0 = k * READS / OPS, r1 = (k + 1) * READS / OPS;
+                        mx_unroll<r1 - r0>([&](auto dd) {
+                            constexpr int e = r0 + decltype(dd)::value;
+                            if constexpr (e < NT) fw[fb ^ 1][e] = fragw(from, nt, e);
+                            else fx[fb ^ 1][e - NT] = fragx(from, nt, e - NT);
+                        });
+                    }
+                    if constexpr (LOAD) {
+                        constexpr int l0 = k * LOADS / OPS, l1 = (k + 1) * LOADS / OPS;
+                        mx_unroll<l1 - l0>([&](auto dd) { load1(fill, l0 + decltype(dd)::value); });
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                if constexpr (LOAD) advance();
             });
-            if (s + 1 < steps) {
-                take();
-                if (s + 2 < steps) scales(s + 2);
-            }
-            if constexpr (RING == 2) { const int keep = at; at = next; next = keep; fill = at; }
-            else { const int keep = at; at = next; next = fill; fill = keep; }
-        }
+            if constexpr (MORE > 0) take();
+            const int keep = at;
+            at = next;
+            if constexpr (RING == 2) { next = keep; fill = at; }
+            else { next = fill; fill = keep; }
+        };
+        int s = 0;
+        for (; s + 2 < steps; ++s) step(s, mx_int<2>{});
+        if (s + 1 < steps) step(s++, mx_int<1>{});
+        step(s, mx_int<0>{});
     }
     for (int b = steps * STEP; b < a.nblk; b += 2) {                  // the rest of K, two blocks at a time
         const bool in = b + q < a.nblk;
         const uint4 zero = make_uint4(0, 0, 0, 0);
         mx_i8 fx[MT], fw[NT];
-        uint32_t ra[MT], rw[NT];
+        uint32_t ta[MT], tw[NT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const int64_t row = min(m0 + (wm * MT + i) * 32 + r, a.M - 1);
             const uint8_t* p = a.A + row * a.lda;
             if constexpr (AF == MX_FP4) fx[i] = frag4(in ? *(const uint4*)(p + (int64_t)(b + q) * 16) : zero);
             else fx[i] = frag8(*(const uint4*)(p + (int64_t)b * 32 + q * 16), b + 1 < a.nblk ? *(const uint4*)(p + (int64_t)b * 32 + 32 + q * 16) : zero);
-            ra[i] = in ? asb[aso[i] + b + q] : 127u;
+            ta[i] = in ? asb[aso[i] + b + q] : 127u;
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int64_t row = min(n0 + (wn * NT + j) * 32 + r, a.N - 1);
             fw[j] = frag4(in ? *(const uint4*)(a.W + row * a.ldw + (int64_t)(b + q) * 16) : zero);
-            rw[j] = in ? wsb[wso[j] + b + q] : 127u;
+            tw[j] = in ? wsb[wso[j] + b + q] : 127u;
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], rw[j], ra[i]);
+            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], tw[j], ta[i]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
