@@ -181,6 +181,7 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxArgs a, int strips) {
 // instruction's byte selector walks the sub-steps.  What is left of K behind the whole steps is fetched straight into registers.
 typedef float mx_f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
+typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
 
 // 16 bytes a lane from a wave-uniform base plus a per-lane offset into LDS at a wave-uniform address (lane order); not tracked by the
 // compiler, so that fragment reads of the other buffer do not wait for it: the kernel waits for all of them in front of its barrier
@@ -270,27 +271,55 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     for (int i = 0; i < MT; ++i) aso[i] = (uint32_t)min((int64_t)((wm * MT + i) * 32 + r), a.M - 1 - m0) * (uint32_t)a.ldas;
 #pragma unroll
     for (int j = 0; j < NT; ++j) wso[j] = (uint32_t)min((int64_t)((wn * NT + j) * 32 + r), a.N - 1 - n0) * (uint32_t)a.ldws;
-    constexpr int SD = STEP / 4;                                      // dwords of scales a row and step
-    // raw: as loaded, two steps ahead;  nx: shifted, the next step's;  sa, sw: this step's
-    uint32_t ra[MT][SD], rw[NT][SD], na[MT][SD], nw[NT][SD], sa[MT][SD], sw[NT][SD];
-    auto scales = [&](int step) {
+    // A load of scales touches a cache line a row, so it costs the same for one step's bytes as for 16: those of GS steps are loaded
+    // together (a load a step took a quarter of the kernel's time).  grp: the current group's, as loaded;  far: the next group's;
+    // sa, sw: this step's, shifted to the lane's half;  na, nw: the next step's
+    constexpr int SD = STEP / 4, GS = 4 / SD;                         // dwords of scales a row and step, steps a group
+    uint32_t grpa[MT][4], grpw[NT][4], fara[MT][4], farw[NT][4], na[MT][SD], nw[NT][SD], sa[MT][SD], sw[NT][SD];
+    auto far_group = [&](int step) {
+        const uint8_t *ua = asb + step * STEP, *uw = wsb + step * STEP;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const mx_u128 u = *(const mx_u128*)(ua + aso[i]);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) fara[i][d] = u[d];
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const mx_u128 u = *(const mx_u128*)(uw + wso[j]);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) farw[j][d] = u[d];
+        }
+    };
+    auto take_group = [&]() {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) grpa[i][d] = fara[i][d];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) grpw[j][d] = farw[j][d];
+        }
+    };
+    // one step's bytes, into the group's first place: the steps behind the last whole group
+    auto one_step = [&](int step) {
         const uint8_t *ua = asb + step * STEP, *uw = wsb + step * STEP;
 #pragma unroll
         for (int d = 0; d < SD; ++d) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) ra[i][d] = *(const mx_u32*)(ua + aso[i] + 4 * d);
+            for (int i = 0; i < MT; ++i) grpa[i][d] = *(const mx_u32*)(ua + aso[i] + 4 * d);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) rw[j][d] = *(const mx_u32*)(uw + wso[j] + 4 * d);
+            for (int j = 0; j < NT; ++j) grpw[j][d] = *(const mx_u32*)(uw + wso[j] + 4 * d);
         }
     };
-    // pinned where it stands: moved down, it would wait for loads issued after those it needs
-    auto shift = [&]() {
+    // the next step's scales from place k of `ga`, `gw`; pinned where it stands: moved down, it would wait for loads issued after
+    // those it needs
+    auto shift = [&](const uint32_t (&ga)[MT][4], const uint32_t (&gw)[NT][4], int k) {
 #pragma unroll
         for (int d = 0; d < SD; ++d) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) { na[i][d] = ra[i][d] >> (8 * q); asm volatile("" : "+v"(na[i][d])); }
+            for (int i = 0; i < MT; ++i) { na[i][d] = ga[i][k * SD + d] >> (8 * q); asm volatile("" : "+v"(na[i][d])); }
 #pragma unroll
-            for (int j = 0; j < NT; ++j) { nw[j][d] = rw[j][d] >> (8 * q); asm volatile("" : "+v"(nw[j][d])); }
+            for (int j = 0; j < NT; ++j) { nw[j][d] = gw[j][k * SD + d] >> (8 * q); asm volatile("" : "+v"(nw[j][d])); }
         }
     };
     auto take = [&]() {
@@ -325,22 +354,25 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         mx_i8 fx[2][MT], fw[2][NT];
         load(0);
         if (RING == 3 && steps > 1) load(STAGE);
-        scales(0);
+        const bool grouped = steps >= 2 * GS;
+        if (grouped) { far_group(0); take_group(); }
+        else one_step(0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        shift();
+        shift(grpa, grpw, 0);
         take();
-        if (steps > 1) scales(1);
+        if (!grouped && steps > 1) one_step(1);
         if (RING == 2 && steps > 1) load(STAGE);
 #pragma unroll
         for (int i = 0; i < MT; ++i) fx[0][i] = fragx(0, 0, i);
 #pragma unroll
         for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
         int at = 0, next = STAGE, fill = RING == 3 ? 2 * STAGE : 0;
-        // one step; MORE steps behind it (0, 1 or at least 2) decide what is fetched.  No branch inside: the compiler would move a
+        // one step; MORE steps behind it (0, 1 or at least 2) decide what is fetched; PLACE: the step's place in its group, -1 for a step
+        // behind the last whole group.  No branch inside: the compiler would move a
         // sub-step's multiplications behind it, away from the fetches they hide
-        auto step = [&](int s, auto more) {
-            constexpr int MORE = decltype(more)::value;
+        auto step = [&](int s, auto more, auto place) {
+            constexpr int MORE = decltype(more)::value, PLACE = decltype(place)::value;
             mx_unroll<SUB>([&](auto tt) {
                 constexpr int t = decltype(tt)::value, nt = (t + 1) % SUB, fb = t & 1;
                 constexpr bool LAST = t == SUB - 1;
@@ -350,9 +382,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                     // the wait above covered the next step's scales too: they leave their registers here, in front of any new load
-                    shift();
+                    if constexpr (PLACE == GS - 1) { shift(fara, farw, 0); take_group(); }
+                    else shift(grpa, grpw, PLACE < 0 ? 0 : PLACE + 1);
                     __builtin_amdgcn_sched_barrier(0);
-                    if constexpr (MORE > 1) scales(s + 2);
+                    if constexpr (PLACE == 0) far_group(s + GS);
+                    if constexpr (PLACE < 0 && MORE > 1) one_step(s + 2);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // behind each multiplication one fragment is fetched for the next sub-step and, behind the barrier, one load goes out
@@ -385,9 +419,19 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
             else { next = fill; fill = keep; }
         };
         int s = 0;
-        for (; s + 2 < steps; ++s) step(s, mx_int<2>{});
-        if (s + 1 < steps) step(s++, mx_int<1>{});
-        step(s, mx_int<0>{});
+        for (; s + 2 * GS <= steps; s += GS) mx_unroll<GS>([&](auto place) { step(s + decltype(place)::value, mx_int<2>{}, place); });
+        if (grouped) {                                                // the step behind next is in the group at hand
+#pragma unroll
+            for (int d = 0; d < SD; ++d) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) grpa[i][d] = grpa[i][SD + d];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) grpw[j][d] = grpw[j][SD + d];
+            }
+        }
+        for (; s + 2 < steps; ++s) step(s, mx_int<2>{}, mx_int<-1>{});
+        if (s + 1 < steps) step(s++, mx_int<1>{}, mx_int<-1>{});
+        step(s, mx_int<0>{}, mx_int<-1>{});
     }
     for (int b = steps * STEP; b < a.nblk; b += 2) {                  // the rest of K, two blocks at a time
         const bool in = b + q < a.nblk;
@@ -413,15 +457,54 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], tw[j], ta[i]);
     }
+    // Out through LDS, 32 rows of the wave at a time: a lane holds four columns of one row, whole rows make whole cache lines (stored
+    // straight from the registers this took 18 us a tile, a fifth of the 5120-deep product).  Piece p (16 bytes) of a row lies at p ^ turn(row),
+    // which spreads 16 rows over the banks.
+    constexpr int SZ = ODT == MX_F32 ? 4 : 2, P = 32 * NT * SZ / 16, EL = 16 / SZ;     // pieces a row, elements a piece
+    auto turn = [](int row) { return P >= 16 ? row & 15 : (row / (16 / P)) & (P - 1); };
+    static_assert(WM * WN * 32 * P * 16 <= RING * STAGE, "");
+    uint8_t* mine = smem + wave * (32 * P * 16);
+    const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.ldo * SZ & 15) == 0;
+    const int64_t nw0 = n0 + wn * NT * 32;
+    __syncthreads();                                                  // every wave is done with the ring
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const mx_f4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                mx_out4<ODT>(a, m0 + (wm * MT + i) * 32 + r, n0 + (wn * NT + j) * 32 + 8 * g + 4 * q, v);
+                const int c = 32 * j + 8 * g + 4 * q;                 // the wave's column
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+                if (a.bias) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += a.bias[min(nw0 + c + e, a.N - 1)];
+                }
+                uint8_t* to = mine + r * (P * 16) + ((c * SZ / 16) ^ turn(r)) * 16 + (c * SZ & 15);
+                if constexpr (ODT == MX_F32) *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
+                else *(uint2*)to = make_uint2(mx_pair<ODT>(v[0], v[1]), mx_pair<ODT>(v[2], v[3]));
             }
+        const int64_t mw0 = m0 + (wm * MT + i) * 32;
+#pragma unroll
+        for (int k = 0; k < P / 2; ++k) {
+            const int row = (k * 64 + lane) / P, piece = (k * 64 + lane) % P;
+            const uint4 u = *(const uint4*)(mine + row * (P * 16) + (piece ^ turn(row)) * 16);
+            const int64_t m = mw0 + row, n = nw0 + piece * EL;
+            if (m >= a.M || n >= a.N) continue;
+            uint8_t* to = (uint8_t*)a.out + (m * a.ldo + n) * SZ;
+            if (wide && n + EL <= a.N) *(uint4*)to = u;
+            else {
+                const uint32_t d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < EL; ++e)
+                    if (n + e < a.N) {
+                        if constexpr (SZ == 4) ((uint32_t*)to)[e] = d[e];
+                        else ((uint16_t*)to)[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
+                    }
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
