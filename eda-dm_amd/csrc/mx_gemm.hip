@@ -186,12 +186,12 @@ typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
 // 16 bytes a lane from a wave-uniform base plus a per-lane offset into LDS at a wave-uniform address (lane order); not tracked by the
 // compiler, so that fragment reads of the other buffer do not wait for it: the kernel waits for all of them in front of its barrier
 __device__ __forceinline__ void mx_dma16(const void* base, uint32_t voff, uint32_t lds) {
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(base), "s"(lds)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
+
+// everything in flight from memory has arrived (LDS: and from LDS); a form the compiler knows, so that it does not wait again for loads
+// that it would find behind newer ones
+template <bool LDS> __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(LDS ? 0x0070 : 0x0f70); }
 
 // a wave-uniform address in scalar registers
 __device__ __forceinline__ const void* mx_uniform(const void* p) {
@@ -220,6 +220,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     constexpr int ABYTES = BM * 128, WBYTES = BN * WROW, STAGE = ABYTES + WBYTES;
     constexpr int RING = AF == MX_FP4 ? 2 : 3;                        // steps' operands in LDS
     constexpr int AI = ABYTES / (THREADS * 16), WI = WBYTES / (THREADS * 16);   // load instructions a wave
+    constexpr int LOADS = AI + WI, EARLY = AF == MX_FP4 ? LOADS / 2 : LOADS;                  // those sent out behind the barrier of the step before
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -272,64 +273,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
     for (int j = 0; j < NT; ++j) wso[j] = (uint32_t)min((int64_t)((wn * NT + j) * 32 + r), a.N - 1 - n0) * (uint32_t)a.ldws;
     // A load of scales touches a cache line a row, so it costs the same for one step's bytes as for 16: those of GS steps are loaded
-    // together (a load a step took a quarter of the kernel's time).  grp: the current group's, as loaded;  far: the next group's;
-    // sa, sw: this step's, shifted to the lane's half;  na, nw: the next step's
-    constexpr int SD = STEP / 4, GS = 4 / SD;                         // dwords of scales a row and step, steps a group
-    uint32_t grpa[MT][4], grpw[NT][4], fara[MT][4], farw[NT][4], na[MT][SD], nw[NT][SD], sa[MT][SD], sw[NT][SD];
-    auto far_group = [&](int step) {
-        const uint8_t *ua = asb + step * STEP, *uw = wsb + step * STEP;
+    // together (a load a step took a quarter of the kernel's time).  Rows e < MT are a's, the others w's.  grp: the current group's, as
+    // loaded;  far: the next group's;  sc: this step's, shifted to the lane's half;  nx: the next step's
+    constexpr int SD = STEP / 4;                                      // dwords of scales a row and step
+    constexpr int GS = 4 / SD, ROWS = MT + NT;                        // steps a group
+    uint32_t grp[ROWS][4], far[ROWS][4], nx[ROWS][SD], sc[ROWS][SD];
+    auto row_at = [&](int e, int step) { return (e < MT ? asb + step * STEP + aso[e < MT ? e : 0] : wsb + step * STEP + wso[e < MT ? 0 : e - MT]); };
+    auto far1 = [&](int e, int step) {
+        const mx_u128 u = *(const mx_u128*)row_at(e, step);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const mx_u128 u = *(const mx_u128*)(ua + aso[i]);
-#pragma unroll
-            for (int d = 0; d < 4; ++d) fara[i][d] = u[d];
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const mx_u128 u = *(const mx_u128*)(uw + wso[j]);
-#pragma unroll
-            for (int d = 0; d < 4; ++d) farw[j][d] = u[d];
-        }
-    };
-    auto take_group = [&]() {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) grpa[i][d] = fara[i][d];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) grpw[j][d] = farw[j][d];
-        }
+        for (int d = 0; d < 4; ++d) far[e][d] = u[d];
     };
     // one step's bytes, into the group's first place: the steps behind the last whole group
-    auto one_step = [&](int step) {
-        const uint8_t *ua = asb + step * STEP, *uw = wsb + step * STEP;
+    auto one1 = [&](int e, int step) {
 #pragma unroll
-        for (int d = 0; d < SD; ++d) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) grpa[i][d] = *(const mx_u32*)(ua + aso[i] + 4 * d);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) grpw[j][d] = *(const mx_u32*)(uw + wso[j] + 4 * d);
-        }
+        for (int d = 0; d < SD; ++d) grp[e][d] = *(const mx_u32*)(row_at(e, step) + 4 * d);
     };
-    // the next step's scales from place k of `ga`, `gw`; pinned where it stands: moved down, it would wait for loads issued after
-    // those it needs
-    auto shift = [&](const uint32_t (&ga)[MT][4], const uint32_t (&gw)[NT][4], int k) {
+    // the next step's scales from place k of a group, then (NEW) the next group in the old one's place
+    auto shift1 = [&](int e, int k, bool turn_over) {
 #pragma unroll
-        for (int d = 0; d < SD; ++d) {
+        for (int d = 0; d < SD; ++d) nx[e][d] = (turn_over ? far[e][d] : grp[e][k * SD + d]) >> (8 * q);
+        if (turn_over) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) { na[i][d] = ga[i][k * SD + d] >> (8 * q); asm volatile("" : "+v"(na[i][d])); }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) { nw[j][d] = gw[j][k * SD + d] >> (8 * q); asm volatile("" : "+v"(nw[j][d])); }
+            for (int d = 0; d < 4; ++d) grp[e][d] = far[e][d];
         }
     };
     auto take = [&]() {
 #pragma unroll
-        for (int d = 0; d < SD; ++d) {
+        for (int e = 0; e < ROWS; ++e)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) sa[i][d] = na[i][d];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) sw[j][d] = nw[j][d];
-        }
+            for (int d = 0; d < SD; ++d) sc[e][d] = nx[e][d];
     };
     // fragment i of a (j of w) of sub-step t in ring slot `at` (bytes): the swizzle depends on the lane alone, so that all rows of a
     // sub-step share one address
@@ -353,16 +326,26 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     if (steps) {
         mx_i8 fx[2][MT], fw[2][NT];
         load(0);
-        if (RING == 3 && steps > 1) load(STAGE);
         const bool grouped = steps >= 2 * GS;
-        if (grouped) { far_group(0); take_group(); }
-        else one_step(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) {
+            if (grouped) far1(e, 0);
+            else one1(e, 0);
+        }
+        mx_wait<RING == 2>();
         __builtin_amdgcn_s_barrier();
-        shift(grpa, grpw, 0);
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) shift1(e, 0, grouped);
         take();
-        if (!grouped && steps > 1) one_step(1);
-        if (RING == 2 && steps > 1) load(STAGE);
+        if (!grouped && steps > 1) {
+#pragma unroll
+            for (int e = 0; e < ROWS; ++e) one1(e, 1);
+        }
+        if (steps > 1) {
+#pragma unroll
+            for (int l = 0; l < EARLY; ++l) load1(STAGE, l);
+            if (EARLY == LOADS) advance();
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) fx[0][i] = fragx(0, 0, i);
 #pragma unroll
@@ -377,40 +360,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                 constexpr int t = decltype(tt)::value, nt = (t + 1) % SUB, fb = t & 1;
                 constexpr bool LAST = t == SUB - 1;
                 if constexpr (LAST && MORE > 0) {
-                    if constexpr (RING == 2) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    asm volatile("" ::: "memory");
+                    mx_wait<RING == 2>();
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
-                    // the wait above covered the next step's scales too: they leave their registers here, in front of any new load
-                    if constexpr (PLACE == GS - 1) { shift(fara, farw, 0); take_group(); }
-                    else shift(grpa, grpw, PLACE < 0 ? 0 : PLACE + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if constexpr (PLACE == 0) far_group(s + GS);
-                    if constexpr (PLACE < 0 && MORE > 1) one_step(s + 2);
-                    __builtin_amdgcn_sched_barrier(0);
                 }
-                // behind each multiplication one fragment is fetched for the next sub-step and, behind the barrier, one load goes out
+                // behind each multiplication: a fragment for the next sub-step; a load instruction, of the step after next behind the
+                // barrier, what is left of the next step's in the first sub-step; a row of the next step's scales (awaited at the
+                // barrier) and the load of a row of scales
                 const int from = LAST ? next : at;
-                constexpr bool FETCH = !LAST || MORE > 0, LOAD = LAST && MORE > 1;
-                constexpr int OPS = MT * NT, READS = MT + NT, LOADS = AI + WI;
+                constexpr int OPS = MT * NT, READS = !LAST || MORE > 0 ? MT + NT : 0, SHIFTS = LAST && MORE > 0 ? ROWS : 0;
+                constexpr int LOW = LAST ? 0 : EARLY, FILL = LAST && MORE > 1 ? EARLY : t == 0 && MORE > 0 ? LOADS - EARLY : 0;
                 mx_unroll<OPS>([&](auto kk) {
                     constexpr int k = decltype(kk)::value, i = k / NT, j = k % NT;
-                    acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sw[j][t / 2], sa[i][t / 2]);
-                    if constexpr (FETCH) {
-                        constexpr int r0 = k * READS / OPS, r1 = (k + 1) * READS / OPS;
-                        mx_unroll<r1 - r0>([&](auto dd) {
-                            constexpr int e = r0 + decltype(dd)::value;
-                            if constexpr (e < NT) fw[fb ^ 1][e] = fragw(from, nt, e);
-                            else fx[fb ^ 1][e - NT] = fragx(from, nt, e - NT);
-                        });
-                    }
-                    if constexpr (LOAD) {
-                        constexpr int l0 = k * LOADS / OPS, l1 = (k + 1) * LOADS / OPS;
-                        mx_unroll<l1 - l0>([&](auto dd) { load1(fill, l0 + decltype(dd)::value); });
-                    }
+                    acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sc[MT + j][t / 2], sc[i][t / 2]);
+                    mx_unroll<(k + 1) * READS / OPS - k * READS / OPS>([&](auto dd) {
+                        constexpr int e = k * READS / OPS + decltype(dd)::value;
+                        if constexpr (e < NT) fw[fb ^ 1][e] = fragw(from, nt, e);
+                        else fx[fb ^ 1][e - NT] = fragx(from, nt, e - NT);
+                    });
+                    mx_unroll<(k + 1) * FILL / OPS - k * FILL / OPS>([&](auto dd) { load1(LAST ? fill : next, LOW + k * FILL / OPS + decltype(dd)::value); });
+                    mx_unroll<(k + 1) * SHIFTS / OPS - k * SHIFTS / OPS>([&](auto dd) {
+                        constexpr int e = k * SHIFTS / OPS + decltype(dd)::value;
+                        shift1(e, PLACE < 0 ? 0 : PLACE + 1, PLACE == GS - 1);
+                        if constexpr (PLACE == 0) far1(e, s + GS);
+                        if constexpr (PLACE < 0 && MORE > 1) one1(e, s + 2);
+                    });
                     __builtin_amdgcn_sched_barrier(0);
                 });
-                if constexpr (LOAD) advance();
+                if constexpr (FILL && (LAST ? EARLY == LOADS : true)) advance();
             });
             if constexpr (MORE > 0) take();
             const int keep = at;
@@ -424,9 +402,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
             for (int d = 0; d < SD; ++d) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) grpa[i][d] = grpa[i][SD + d];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) grpw[j][d] = grpw[j][SD + d];
+                for (int e = 0; e < ROWS; ++e) grp[e][d] = grp[e][SD + d];
             }
         }
         for (; s + 2 < steps; ++s) step(s, mx_int<2>{}, mx_int<-1>{});
