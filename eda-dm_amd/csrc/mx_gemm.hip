@@ -90,76 +90,140 @@ template <int ODT> __device__ __forceinline__ void mx_out4(const MxArgs& a, int6
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// A workgroup owns 16 NT columns and 16 MT rows; its waves take the K-steps of 128 in turn, fetch their operands straight into
-// registers (UK steps of them in flight) and add their sums in LDS in the order of the waves.  Bound by reading w once.
-template <int AF, int MT, int NT, int UK, bool EXACT, int ODT>
-__global__ __launch_bounds__(512) void k_mx_rows(MxArgs a, int strips) {
-    constexpr int WAVES = 8;
-    __shared__ mx_f4 red[WAVES][MT * NT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+// A workgroup owns 16 MT rows and 16 NT columns; its waves (as many as the launch gives it) take pairs of K-steps of 128 in turn, so
+// that every cache line of w (128 bytes = a pair of a row) is read by one wave, fetch their operands straight into registers, a pair
+// ahead of the one they multiply, and add their sums in LDS in the order of the waves.  Bound by reading w once.
+typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
+typedef uint32_t mx_u64 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
+
+template <int AF, int MT, int NT> struct MxPair {                     // a lane's operands of two K-steps
+    uint4 w[NT][2], x[MT][AF == MX_FP4 ? 2 : 4];
+    uint32_t sw[NT][2], sa[MT][2];
+};
+
+template <int AF, int MT, int NT, int MAXW, bool EXACT, int ODT>
+__global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
+    constexpr int TILES = MT * NT, CH = TILES < 4 ? TILES : 4;        // tiles summed at a time
+    constexpr int NX = AF == MX_FP4 ? 2 : 4;
+    __shared__ mx_f4 red[MAXW][CH][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
+    const int r = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)(blockIdx.x % strips) * (16 * NT), m0 = (int64_t)(blockIdx.x / strips) * (16 * MT);
-    const int steps = (a.nblk + 3) / 4;
     const uint8_t *wp[NT], *wsp[NT], *ap[MT], *asp[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int64_t n = min(n0 + 16 * j + r, a.N - 1);              // rows past the end: read the last one, store nothing
-        wp[j] = a.W + n * a.ldw + q * 16;
-        wsp[j] = a.Ws + n * a.ldws + q;
+        wp[j] = a.W + n * a.ldw;
+        wsp[j] = a.Ws + n * a.ldws;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t m = min(m0 + 16 * i + r, a.M - 1);
-        ap[i] = a.A + m * a.lda + q * 16;
-        asp[i] = a.As + m * a.ldas + q;
+        ap[i] = a.A + m * a.lda;
+        asp[i] = a.As + m * a.ldas;
     }
+    // a whole pair: eight blocks; the 16-byte pieces of a lane are blocks q and 4 + q (4 bits), halves of blocks (8 bits)
+    auto fetch = [&](int pair, MxPair<AF, MT, NT>& f) {
+        const int64_t b = (int64_t)pair * 8;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) f.w[j][u] = *(const uint4*)(wp[j] + b * 16 + u * 64 + q * 16);
+            const mx_u64 s = *(const mx_u64*)(wsp[j] + b);
+            f.sw[j][0] = s[0];
+            f.sw[j][1] = s[1];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int u = 0; u < NX; ++u) f.x[i][u] = *(const uint4*)(ap[i] + b * (NX * 8) + u * 64 + q * 16);
+            const mx_u64 s = *(const mx_u64*)(asp[i] + b);
+            f.sa[i][0] = s[0];
+            f.sa[i][1] = s[1];
+        }
+    };
+    // the last, short pair: blocks past the end are read from the last one and put to zero under a scale of 1
+    auto fetch_end = [&](int pair, MxPair<AF, MT, NT>& f) {
+        const int b = pair * 8, last = a.nblk - 1;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int k = b + 4 * u + q, kc = min(k, last);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint4 v = *(const uint4*)(wp[j] + (int64_t)kc * 16);
+                const uint32_t s = wsp[j][kc];
+                f.w[j][u] = k <= last ? v : zero;
+                f.sw[j][u] = (k <= last ? s : 127u) << (8 * q);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint32_t s = asp[i][kc];
+                f.sa[i][u] = (k <= last ? s : 127u) << (8 * q);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NX; ++u) {
+            const int k = AF == MX_FP4 ? b + 4 * u + q : b + 2 * u + (q >> 1), kc = min(k, last);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint4 v = *(const uint4*)(ap[i] + (AF == MX_FP4 ? (int64_t)kc * 16 : (int64_t)kc * 32 + (q & 1) * 16));
+                f.x[i][u] = k <= last ? v : zero;
+            }
+        }
+    };
     mx_f4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = mx_f4{0, 0, 0, 0};
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int s0 = wave; s0 < steps; s0 += WAVES * UK) {
-        uint4 w[UK][NT], x[UK][MT], y[UK][MT];
-        uint32_t sw[UK][NT], sa[UK][MT];
+    auto multiply = [&](const MxPair<AF, MT, NT>& f) {
 #pragma unroll
-        for (int u = 0; u < UK; ++u) {
-            const int b = (s0 + u * WAVES) * 4;                       // first block of the step
-            const bool in = b + q < a.nblk;                           // blocks past the end: zeros under any finite scale
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                w[u][j] = in ? *(const uint4*)(wp[j] + (int64_t)b * 16) : zero;
-                sw[u][j] = in ? wsp[j][b] : 127u;
-            }
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if constexpr (AF == MX_FP4) x[u][i] = in ? *(const uint4*)(ap[i] + (int64_t)b * 16) : zero;
-                else {
-                    x[u][i] = b + (q >> 1) < a.nblk ? *(const uint4*)(ap[i] + (int64_t)b * 32) : zero;
-                    y[u][i] = b + 2 + (q >> 1) < a.nblk ? *(const uint4*)(ap[i] + (int64_t)b * 32 + 64) : zero;
-                }
-                sa[u][i] = in ? asp[i][b] : 127u;
+                const mx_i8 fa = AF == MX_FP4 ? frag4(f.x[i][u]) : frag8(f.x[i][NX / 2 * u], f.x[i][NX / 2 * u + NX / 2 - 1]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    acc[i][j] = mx_mma16<AF, EXACT>(frag4(f.w[j][u]), fa, acc[i][j], f.sw[j][u] >> (8 * q), f.sa[i][u] >> (8 * q));
             }
+    };
+    const int whole = a.nblk / 8;
+    int p = wave;
+    if (p < whole) {
+        MxPair<AF, MT, NT> f[2];
+        fetch(p, f[0]);
+        while (true) {
+            if (p + waves < whole) fetch(p + waves, f[1]);
+            multiply(f[0]);
+            p += waves;
+            if (p >= whole) break;
+            if (p + waves < whole) fetch(p + waves, f[0]);
+            multiply(f[1]);
+            p += waves;
+            if (p >= whole) break;
         }
-#pragma unroll
-        for (int u = 0; u < UK; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const mx_i8 fa = AF == MX_FP4 ? frag4(x[u][i]) : frag8(x[u][i], y[u][i]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma16<AF, EXACT>(frag4(w[u][j]), fa, acc[i][j], sw[u][j], sa[u][i]);
-            }
+    }
+    if (p == whole && whole * 8 < a.nblk) {
+        MxPair<AF, MT, NT> f;
+        fetch_end(p, f);
+        multiply(f);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int c = 0; c < TILES; c += CH) {
+        if (c) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NT; ++j) red[wave][i * NT + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int e = threadIdx.x; e < MT * NT * 64; e += WAVES * 64) {
-        const int tile = e >> 6, l = e & 63;
-        mx_f4 v = red[0][tile][l];
-#pragma unroll
-        for (int k = 1; k < WAVES; ++k) v += red[k][tile][l];
-        mx_out4<ODT>(a, m0 + 16 * (tile / NT) + (l & 15), n0 + 16 * (tile % NT) + 4 * (l >> 4), v);
+        for (int t = 0; t < CH; ++t)
+            if (c + t < TILES) red[wave][t][lane] = acc[(c + t) / NT][(c + t) % NT];
+        __syncthreads();
+        for (int e = threadIdx.x; e < CH * 64; e += blockDim.x) {
+            const int t = e >> 6, l = e & 63, tile = c + t;
+            if (tile >= TILES) break;
+            mx_f4 v = red[0][t][l];
+            for (int k = 1; k < waves; ++k) v += red[k][t][l];
+            mx_out4<ODT>(a, m0 + 16 * (tile / NT) + (l & 15), n0 + 16 * (tile % NT) + 4 * (l >> 4), v);
+        }
     }
 }
 
@@ -180,8 +244,6 @@ __global__ __launch_bounds__(512) void k_mx_rows(MxArgs a, int strips) {
 // Scales stay in registers: a lane holds the four (eight) bytes of its row for a step, shifted by its half of the wave, so that the
 // instruction's byte selector walks the sub-steps.  What is left of K behind the whole steps is fetched straight into registers.
 typedef float mx_f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
-typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
 
 // 16 bytes a lane from a wave-uniform base plus a per-lane offset into LDS at a wave-uniform address (lane order); not tracked by the
 // compiler, so that fragment reads of the other buffer do not wait for it: the kernel waits for all of them in front of its barrier
@@ -484,17 +546,24 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-template <int AF, bool EXACT, int ODT> static int launch_rows(const MxArgs& a, hipStream_t st) {
-    const int64_t mt = (a.M + 15) / 16;
-    const int m = mt >= 4 ? 4 : mt == 3 ? 3 : (int)mt;
-    const int64_t strips = (a.N + 15) / 16, chunks = (mt + m - 1) / m;
-    if (strips > 0x7fffffff || strips * chunks > 0x7fffffff) return EDADM_EINVAL;
-    const unsigned grid = (unsigned)(strips * chunks);
-    if (m == 1) k_mx_rows<AF, 1, 1, 5, EXACT, ODT><<<grid, 512, 0, st>>>(a, (int)strips);
-    else if (m == 2) k_mx_rows<AF, 2, 1, 3, EXACT, ODT><<<grid, 512, 0, st>>>(a, (int)strips);
-    else if (m == 3) k_mx_rows<AF, 3, 1, 2, EXACT, ODT><<<grid, 512, 0, st>>>(a, (int)strips);
-    else k_mx_rows<AF, 4, 1, 2, EXACT, ODT><<<grid, 512, 0, st>>>(a, (int)strips);
+template <int AF, int MT, int NT, bool EXACT, int ODT> static int launch_rows1(const MxArgs& a, hipStream_t st) {
+    constexpr int MAXW = MT * NT <= 2 ? 16 : 8;
+    const int64_t strips = (a.N + 16 * NT - 1) / (16 * NT), chunks = (a.M + 16 * MT - 1) / (16 * MT);
+    if (strips > 0x7fffffff || chunks > 0x7fffffff || strips * chunks > 0x7fffffff) return EDADM_EINVAL;
+    // waves: two pairs each (one is fetched while the other multiplies) as far as they go
+    const int pairs = (a.nblk + 7) / 8, each = pairs > 2 * MAXW ? (pairs + MAXW - 1) / MAXW : pairs > 4 ? 2 : 1;
+    const int waves = (pairs + each - 1) / each;
+    k_mx_rows<AF, MT, NT, MAXW, EXACT, ODT><<<(unsigned)(strips * chunks), 64 * waves, 0, st>>>(a, (int)strips);
     return edadm_launch_status();
+}
+template <int AF, bool EXACT, int ODT> static int launch_rows(const MxArgs& a, hipStream_t st) {
+    // rows of a are read by every strip of columns: the strip is as wide as the rows are many, as long as there are strips for the CUs
+    const int mt = (int)((a.M + 15) / 16);
+    const bool many = a.N >= 64 * 96;
+    if (mt == 1) return launch_rows1<AF, 1, 1, EXACT, ODT>(a, st);
+    if (mt == 2) return launch_rows1<AF, 2, 2, EXACT, ODT>(a, st);
+    if (mt == 3) return many ? launch_rows1<AF, 3, 4, EXACT, ODT>(a, st) : launch_rows1<AF, 3, 2, EXACT, ODT>(a, st);
+    return many ? launch_rows1<AF, 4, 4, EXACT, ODT>(a, st) : launch_rows1<AF, 4, 2, EXACT, ODT>(a, st);
 }
 
 template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static int launch_tile(const MxArgs& a, hipStream_t st) {

@@ -72,13 +72,19 @@ CALLS = None
 TRACE_HOOK = None
 
 
+_fns = {}
+
+
 def call(name, *args):
     """Invoke an int-returning entry point; non-zero status raises."""
     if CALLS is not None:
         CALLS[name] = CALLS.get(name, 0) + 1
     if TRACE_HOOK is not None:
         TRACE_HOOK(name, args)
-    rc = getattr(load(), name)(*args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != 0:
         raise EdadmError("%s failed with status %d" % (name, rc))
 

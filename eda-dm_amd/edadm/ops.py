@@ -1003,32 +1003,35 @@ def softmax_f32(s2d):
 
 
 # ------------------------------------------------------------------------------ microscaled (MX) formats
+# Calls of one token are bound by the host: these wrappers look at each tensor once, take the raw stream handle and allocate nothing but
+# their outputs.
 _MX_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MX_FMT = {"mxfp4": 4, "mxfp8": 8}
 _MX_PITCH = {"mxfp4": 16, "mxfp8": 32}      # code bytes of a block of 32 elements
 
 
 def _mx_fmt(fmt):
-    if fmt not in _MX_FMT:
+    f = _MX_FMT.get(fmt) if isinstance(fmt, str) else None
+    if f is None:
         raise lib.EdadmError("microscaled format 'mxfp4' or 'mxfp8' expected, got %r" % (fmt,))
-    return _MX_FMT[fmt]
+    return f
 
 
 def _mx_dt(t):
     dt = _MX_DT.get(t.dtype)
     if dt is None:
         raise lib.EdadmError("expected float32, bfloat16 or float16, got %s" % t.dtype)
-    if not t.is_cuda:
-        raise lib.EdadmError("edadm ops need device tensors (no CPU fallback)")
     return dt
 
 
 def _mx_rows(t):
-    """(t as 2-D rows of unit stride, rows, cols, row pitch): a view where the strides allow one -- any pitch, any alignment -- else a
-    copy.  A pitch below the row length (an expanded dimension) is copied too."""
+    """(t as rows of unit stride, rows, cols, row pitch): t itself or a view where the strides allow one -- any pitch, any alignment --
+    else a copy.  A pitch below the row length (an expanded dimension) is copied too."""
     cols = t.shape[-1] if t.dim() else 0
     if cols < 1:
         raise lib.EdadmError("rows of at least one element expected, got shape %s" % (tuple(t.shape),))
+    if t.is_contiguous():
+        return t, t.numel() // cols, cols, cols
     r = t if t.dim() == 2 else t.reshape(-1, cols)
     rows, ld = r.shape[0], r.stride(0)
     if (cols > 1 and r.stride(1) != 1) or (rows > 1 and ld < cols):
@@ -1037,35 +1040,32 @@ def _mx_rows(t):
     return r, rows, cols, ld if rows > 1 else cols
 
 
-class _MxOn:
-    """Launch on the tensors' own device, whatever the current one is; every tensor of the call has to be there."""
-    __slots__ = ("guard",)
-
-    def __init__(self, first, *others):
-        dev = first.device
-        for t in others:
-            if t is not None and t.device != dev:
-                raise lib.EdadmError("tensors on different devices: %s and %s" % (dev, t.device))
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+def _mx_device(first, *others):
+    """the device index every tensor of a call is on"""
+    dev = first.get_device()
+    if dev < 0:
+        raise lib.EdadmError("edadm ops need device tensors (no CPU fallback)")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise lib.EdadmError("tensors on different devices: %s and %s" % (first.device, t.device))
+    return dev
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _mx_call(dev, name, *args):
+    """launch on the tensors' device, whatever the current one is, and on its current stream"""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
+        lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            lib.call(name, *args, stream)
 
 
 class MXTensor:
     """A microscaled tensor: rows of `cols` elements in blocks of 32, each block under one power-of-two scale.
     codes: uint8 [..., blocks * 16] (fmt 'mxfp4': e2m1, two to a byte, the first in the low nibble) or [..., blocks * 32] ('mxfp8': e4m3);
     scales: uint8 [..., blocks], the biased exponent b of the scale 2^(b - 127), 255 = NaN.  The elements behind `cols` in a row's last
-    block are zero codes: mx_gemm multiplies whole blocks.  Code rows are 16-byte aligned."""
+    block are zero codes: mx_gemm multiplies whole blocks."""
     __slots__ = ("codes", "scales", "cols", "fmt")
 
     def __init__(self, codes, scales, cols, fmt):
@@ -1073,9 +1073,10 @@ class MXTensor:
         nb = (cols + 31) // 32
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise lib.EdadmError("codes and scales are uint8 tensors, got %s and %s" % (codes.dtype, scales.dtype))
-        if cols < 1 or codes.shape[-1] != nb * _MX_PITCH[fmt] or scales.shape[-1] != nb or codes.shape[:-1] != scales.shape[:-1]:
+        cs, ss = codes.shape, scales.shape
+        if cols < 1 or cs[-1] != nb * _MX_PITCH[fmt] or ss[-1] != nb or cs[:-1] != ss[:-1]:
             raise lib.EdadmError("%s rows of %d elements have %d code bytes and %d scales, got %s and %s"
-                                 % (fmt, cols, nb * _MX_PITCH[fmt], nb, tuple(codes.shape), tuple(scales.shape)))
+                                 % (fmt, cols, nb * _MX_PITCH[fmt], nb, tuple(cs), tuple(ss)))
         self.codes, self.scales, self.cols, self.fmt = codes, scales, cols, fmt
 
     @property
@@ -1085,20 +1086,23 @@ class MXTensor:
     def _rows(self):
         """(codes, code pitch, scales, scale pitch, rows), rows of unit stride; code rows the kernels cannot read in place (not 16-byte
         aligned) are copied"""
-        c, rows, _, ldc = _mx_rows(self.codes)
+        c, rows, n, ldc = _mx_rows(self.codes)
         s, _, _, lds = _mx_rows(self.scales)
-        if not c.is_cuda or not s.is_cuda:
-            raise lib.EdadmError("edadm ops need device tensors (no CPU fallback)")
-        if c.data_ptr() % 16 or ldc % 16:
+        if c.data_ptr() & 15 or ldc & 15:
             c = c.clone(memory_format=torch.contiguous_format)
-            ldc = c.shape[1]
+            ldc = n
         return c, ldc, s, lds, rows
 
 
-def _mx_empty(shape, cols, fmt, device):
+def _mx_new(x, cols, fmt):
+    """an MXTensor of x's shape for a kernel to fill"""
     nb = (cols + 31) // 32
-    return (torch.empty(tuple(shape[:-1]) + (nb * _MX_PITCH[fmt],), dtype=torch.uint8, device=device),
-            torch.empty(tuple(shape[:-1]) + (nb,), dtype=torch.uint8, device=device))
+    lead = x.shape[:-1]
+    q = MXTensor.__new__(MXTensor)
+    q.codes = x.new_empty(lead + (nb * _MX_PITCH[fmt],), dtype=torch.uint8)
+    q.scales = x.new_empty(lead + (nb,), dtype=torch.uint8)
+    q.cols, q.fmt = cols, fmt
+    return q
 
 
 def mx_quantize(x, fmt):
@@ -1106,31 +1110,32 @@ def mx_quantize(x, fmt):
     2^(floor(log2 max|x|) - 2) ('mxfp4') or 2^(.. - 8) ('mxfp8'), elements are rounded to nearest even and saturate at 6 / 448; a block that
     holds an infinity or NaN reads back as NaN."""
     f, dt = _mx_fmt(fmt), _mx_dt(x)
+    dev = _mx_device(x)
     r, rows, cols, ld = _mx_rows(x)
-    codes, scales = _mx_empty(x.shape, cols, fmt, x.device)
-    with _MxOn(x):
-        lib.call("edadm_mx_quantize", _ptr(r), ld, dt, _ptr(codes), codes.shape[-1], _ptr(scales), scales.shape[-1], rows, cols, f, _stream())
-    return MXTensor(codes, scales, cols, fmt)
+    q = _mx_new(x, cols, fmt)
+    _mx_call(dev, "edadm_mx_quantize", r.data_ptr(), ld, dt, q.codes.data_ptr(), q.codes.shape[-1], q.scales.data_ptr(), q.scales.shape[-1],
+             rows, cols, f)
+    return q
 
 
 def mx_dequantize(q, dtype=torch.float32):
     """MXTensor -> the values it stands for [..., cols], rounded once to `dtype` (exact in fp32)."""
     if dtype not in _MX_DT:
         raise lib.EdadmError("expected float32, bfloat16 or float16, got %s" % dtype)
+    dev = _mx_device(q.codes, q.scales)
     c, ldc, s, lds, rows = q._rows()
     out = torch.empty(q.shape, dtype=dtype, device=c.device)
-    with _MxOn(c, s):
-        lib.call("edadm_mx_dequantize", _ptr(c), ldc, _ptr(s), lds, _MX_FMT[q.fmt], _ptr(out), q.cols, _MX_DT[dtype], rows, q.cols, _stream())
+    _mx_call(dev, "edadm_mx_dequantize", c.data_ptr(), ldc, s.data_ptr(), lds, _MX_FMT[q.fmt], out.data_ptr(), q.cols, _MX_DT[dtype], rows, q.cols)
     return out
 
 
 def mx_fake_quant_fwd(x, fmt):
     """what mx_dequantize(mx_quantize(x)) gives, in x's type, in one pass (train_ops.mx_fake_quant is the differentiable form)"""
     f, dt = _mx_fmt(fmt), _mx_dt(x)
+    dev = _mx_device(x)
     r, rows, cols, ld = _mx_rows(x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _MxOn(x):
-        lib.call("edadm_mx_fake_quant_fwd", _ptr(r), ld, dt, _ptr(out), cols, rows, cols, f, _stream())
+    out = x.new_empty(x.shape)
+    _mx_call(dev, "edadm_mx_fake_quant_fwd", r.data_ptr(), ld, dt, out.data_ptr(), cols, rows, cols, f)
     return out
 
 
@@ -1139,11 +1144,11 @@ def mx_fake_quant_bwd(gy, x, fmt):
     f, dt = _mx_fmt(fmt), _mx_dt(x)
     if gy.shape != x.shape or gy.dtype != x.dtype:
         raise lib.EdadmError("gradient of %s %s for an input of %s %s" % (gy.dtype, tuple(gy.shape), x.dtype, tuple(x.shape)))
+    dev = _mx_device(x, gy)
     r, rows, cols, ld = _mx_rows(x)
     g, _, _, ldg = _mx_rows(gy)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _MxOn(x, gy):
-        lib.call("edadm_mx_fake_quant_bwd", _ptr(g), ldg, _ptr(r), ld, dt, _ptr(out), cols, rows, cols, f, _stream())
+    out = x.new_empty(x.shape)
+    _mx_call(dev, "edadm_mx_fake_quant_bwd", g.data_ptr(), ldg, r.data_ptr(), ld, dt, out.data_ptr(), cols, rows, cols, f)
     return out
 
 
@@ -1152,36 +1157,38 @@ def _rms_args(x, weight, eps, residual):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise lib.EdadmError("residual of %s %s for an input of %s %s" % (residual.dtype, tuple(residual.shape), x.dtype, tuple(x.shape)))
     cols = x.shape[-1] if x.dim() else 0
-    if weight.dim() != 1 or weight.shape[0] != cols or weight.dtype not in (torch.float32, x.dtype):
+    wf32 = weight.dtype == torch.float32
+    if weight.dim() != 1 or weight.shape[0] != cols or not (wf32 or weight.dtype == x.dtype):
         raise lib.EdadmError("a weight of [%d] in float32 or %s expected, got %s %s" % (cols, x.dtype, weight.dtype, tuple(weight.shape)))
-    if cols > lib.load().edadm_rmsnorm_max_cols():
+    if cols > 32768 and cols > lib.load().edadm_rmsnorm_max_cols():
         raise lib.EdadmError("rows of at most %d elements, got %d" % (lib.load().edadm_rmsnorm_max_cols(), cols))
     if not eps >= 0:
         raise lib.EdadmError("eps %r is negative" % (eps,))
-    return dt, weight.contiguous()
+    return dt, weight.contiguous(), 1 if wf32 else 0
 
 
 def rmsnorm_fwd(x, weight, eps, fmt=None, residual=None, fake=False, want_rstd=False):
     """edadm_rmsnorm_fwd: (output, h, rstd): output = y (fmt None), its MXTensor, or (fake) what that stands for in x's type; h is x itself
     without a residual; rstd [rows] fp32 or None"""
-    dt, w = _rms_args(x, weight, eps, residual)
     f = 0 if fmt is None else _mx_fmt(fmt)
+    dt, w, wf32 = _rms_args(x, weight, eps, residual)
+    dev = _mx_device(x, w, residual)
     r, rows, cols, ld = _mx_rows(x)
-    h, ldr, res = x, 0, None
+    h, hp, rp, ldr = x, None, None, 0
     if residual is not None:
         res, _, _, ldr = _mx_rows(residual)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    scales = None
+        h = x.new_empty(x.shape)
+        hp, rp = h.data_ptr(), res.data_ptr()
+    rstd = x.new_empty(rows, dtype=torch.float32) if want_rstd else None
     if f and not fake:
-        out, scales = _mx_empty(x.shape, cols, fmt, x.device)
+        out = _mx_new(x, cols, fmt)
+        op, ldo, sp, lds = out.codes.data_ptr(), out.codes.shape[-1], out.scales.data_ptr(), out.scales.shape[-1]
     else:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _MxOn(x, weight, residual):
-        lib.call("edadm_rmsnorm_fwd", _ptr(r), ld, _ptr(res), ldr, dt, _ptr(w), 1 if w.dtype == torch.float32 else 0,
-                 _ptr(h) if res is not None else None, cols, _ptr(rstd), _ptr(out), out.shape[-1], _ptr(scales),
-                 0 if scales is None else scales.shape[-1], rows, cols, float(eps), f, 1 if fake else 0, _stream())
-    return (out if scales is None else MXTensor(out, scales, cols, fmt)), h, rstd
+        out = x.new_empty(x.shape)
+        op, ldo, sp, lds = out.data_ptr(), cols, None, 0
+    _mx_call(dev, "edadm_rmsnorm_fwd", r.data_ptr(), ld, rp, ldr, dt, w.data_ptr(), wf32, hp, cols, rstd.data_ptr() if want_rstd else None, op, ldo,
+             sp, lds, rows, cols, float(eps), f, 1 if fake else 0)
+    return out, h, rstd
 
 
 def rmsnorm_mx(x, weight, eps, fmt, residual=None):
@@ -1196,25 +1203,25 @@ def rmsnorm_mx(x, weight, eps, fmt, residual=None):
 def rmsnorm_bwd(gy, gh, h, rstd, weight, fmt=None, need_dw=True):
     """(dh, dw) of rmsnorm_fwd (dw None where not needed): gy arrives at the output, gh (or None) at h; dh is the gradient of x and of the
     residual alike"""
-    dt, w = _rms_args(h, weight, 0.0, gh)
+    dt, w, wf32 = _rms_args(h, weight, 0.0, gh)
     if gy.shape != h.shape or gy.dtype != h.dtype:
         raise lib.EdadmError("gradient of %s %s for a stream of %s %s" % (gy.dtype, tuple(gy.shape), h.dtype, tuple(h.shape)))
     f = 0 if fmt is None else _mx_fmt(fmt)
+    dev = _mx_device(h, gy, gh, rstd, w)
     r, rows, cols, ldh = _mx_rows(h)
     if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
         raise lib.EdadmError("rstd [%d] in float32 expected" % rows)
     g, _, _, ldg = _mx_rows(gy)
     up, _, _, ldgh = _mx_rows(gh) if gh is not None else (None, 0, 0, 0)
-    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dh = h.new_empty(h.shape)
     if rows == 0:
         return dh, torch.zeros_like(weight) if need_dw else None
     dw = ws = None
     if need_dw:
-        dw = torch.empty(cols, dtype=weight.dtype, device=h.device)
-        ws = torch.empty(lib.load().edadm_rmsnorm_bwd_ws_floats(rows, cols), dtype=torch.float32, device=h.device)
-    with _MxOn(h, gy, gh, rstd, weight):
-        lib.call("edadm_rmsnorm_bwd", _ptr(g), ldg, _ptr(up), ldgh, _ptr(r), ldh, dt, _ptr(rstd), _ptr(w),
-                 1 if w.dtype == torch.float32 else 0, _ptr(dh), cols, _ptr(dw), _ptr(ws), rows, cols, f, _stream())
+        dw = h.new_empty(cols, dtype=weight.dtype)
+        ws = h.new_empty(lib.load().edadm_rmsnorm_bwd_ws_floats(rows, cols), dtype=torch.float32)
+    _mx_call(dev, "edadm_rmsnorm_bwd", g.data_ptr(), ldg, None if up is None else up.data_ptr(), ldgh, r.data_ptr(), ldh, dt, rstd.data_ptr(),
+             w.data_ptr(), wf32, dh.data_ptr(), cols, dw.data_ptr() if need_dw else None, ws.data_ptr() if need_dw else None, rows, cols, f)
     return dh, dw
 
 
@@ -1227,15 +1234,16 @@ def mx_gemm(a, w, bias=None, dtype=torch.bfloat16):
         raise lib.EdadmError("the second operand is a [N, K] 'mxfp4' weight, got %s %s" % (w.fmt, tuple(w.shape)))
     if a.cols != w.cols:
         raise lib.EdadmError("operands of %d and %d elements a row" % (a.cols, w.cols))
-    if dtype not in _MX_DT:
+    odt = _MX_DT.get(dtype)
+    if odt is None:
         raise lib.EdadmError("expected float32, bfloat16 or float16, got %s" % dtype)
     N = w.codes.shape[0]
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
         raise lib.EdadmError("a contiguous float32 bias of [%d] expected, got %s %s" % (N, bias.dtype, tuple(bias.shape)))
+    dev = _mx_device(a.codes, a.scales, w.codes, w.scales, bias)
     ac, lda, sa, ldas, M = a._rows()
     wc, ldw, sw, ldws, _ = w._rows()
-    out = torch.empty(tuple(a.codes.shape[:-1]) + (N,), dtype=dtype, device=ac.device)
-    with _MxOn(ac, sa, wc, sw, bias):
-        lib.call("edadm_mx_gemm", _ptr(ac), lda, _ptr(sa), ldas, _MX_FMT[a.fmt], _ptr(wc), ldw, _ptr(sw), ldws, M, N, a.cols,
-                 _ptr(bias), _ptr(out), N, _MX_DT[dtype], _stream())
+    out = ac.new_empty(a.codes.shape[:-1] + (N,), dtype=dtype)
+    _mx_call(dev, "edadm_mx_gemm", ac.data_ptr(), lda, sa.data_ptr(), ldas, _MX_FMT[a.fmt], wc.data_ptr(), ldw, sw.data_ptr(), ldws, M, N, a.cols,
+             None if bias is None else bias.data_ptr(), out.data_ptr(), N, odt)
     return out
