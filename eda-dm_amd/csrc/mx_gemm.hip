@@ -10,6 +10,7 @@
 // (and 8 x 4-bit ones within 8 binades) are inside that and sum exactly; e4m3 spans 18 binades, and what falls below is cut off: a
 // relative error of a few 1e-6 of the result, which a 16-bit output's rounding (2e-3) hides.  For a 32-bit output the 8-bit operand is
 // split by the top bit of its exponent into two operands of 8 binades each, both exact, at twice the matrix work.
+#include <math.h>
 #include "mx_common.h"
 #include "../../include/edadm.h"
 
@@ -499,9 +500,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     // straight from the registers this took 18 us a tile, a fifth of the 5120-deep product).  Piece p (16 bytes) of a row lies at p ^ turn(row),
     // which spreads 16 rows over the banks.
     constexpr int SZ = ODT == MX_F32 ? 4 : 2, P = 32 * NT * SZ / 16, EL = 16 / SZ;     // pieces a row, elements a piece
-    auto turn = [](int row) { return P >= 16 ? row & 15 : (row / (16 / P)) & (P - 1); };
-    static_assert(WM * WN * 32 * P * 16 <= RING * STAGE, "");
-    uint8_t* mine = smem + wave * (32 * P * 16);
+    constexpr int PP = P > 16 ? 32 : P > 8 ? 16 : P > 4 ? 8 : 4;                       // a row's room in pieces
+    auto turn = [](int row) { return PP >= 16 ? row & 15 : (row / (16 / PP)) & (PP - 1); };
+    static_assert(WM * WN * 32 * PP * 16 <= RING * STAGE, "");
+    uint8_t* mine = smem + wave * (32 * PP * 16);
     const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.ldo * SZ & 15) == 0;
     const int64_t nw0 = n0 + wn * NT * 32;
     __syncthreads();                                                  // every wave is done with the ring
@@ -519,7 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += a.bias[min(nw0 + c + e, a.N - 1)];
                 }
-                uint8_t* to = mine + r * (P * 16) + ((c * SZ / 16) ^ turn(r)) * 16 + (c * SZ & 15);
+                uint8_t* to = mine + r * (PP * 16) + ((c * SZ / 16) ^ turn(r)) * 16 + (c * SZ & 15);
                 if constexpr (ODT == MX_F32) *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
                 else *(uint2*)to = make_uint2(mx_pair<ODT>(v[0], v[1]), mx_pair<ODT>(v[2], v[3]));
             }
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
         for (int k = 0; k < P / 2; ++k) {
             const int row = (k * 64 + lane) / P, piece = (k * 64 + lane) % P;
-            const uint4 u = *(const uint4*)(mine + row * (P * 16) + (piece ^ turn(row)) * 16);
+            const uint4 u = *(const uint4*)(mine + row * (PP * 16) + (piece ^ turn(row)) * 16);
             const int64_t m = mw0 + row, n = nw0 + piece * EL;
             if (m >= a.M || n >= a.N) continue;
             uint8_t* to = (uint8_t*)a.out + (m * a.ldo + n) * SZ;
@@ -590,10 +592,26 @@ template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hip
     // the tiled kernel's 32-bit row offsets: 256 rows of a and of w under 4 GB
     const bool fits = a.lda < (1 << 23) && a.ldw < (1 << 23) && a.ldas < (1 << 23) && a.ldws < (1 << 23);
     if (a.M <= 64 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
-    const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256), mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (big >= 200) return launch_tile<AF, 2, 2, 4, 4, EXACT, ODT>(a, st);
-    if (mid >= 200) return launch_tile<AF, 2, 2, 2, 2, EXACT, ODT>(a, st);
-    return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
+    // The tile is the one of least cost: tiles a CU x what a tile costs on a full chip, and no less than what one costs alone (both
+    // in units of a 256 x 256 tile on a full chip, 68 us at K = 5120 with 8-bit a, 44 us with 4-bit a; measured over M = 64 .. 8192,
+    // the ratios are the same for both).  4096 x 5120 x 5120: 256 x 256 leaves three quarters of the second round empty (81 us, 4-bit
+    // a), 256 x 192 takes 69;  8192 x 10240 x 5120: 339 against 369 us, 8-bit a;  256 x 5120 x 5120: 64 x 64 takes 15.6 us, 256 x 256 49.
+    static const struct { int bm, bn; float full, alone; } tiles[] = {
+        {256, 256, 1.f, 0.75f}, {256, 192, 0.805f, 0.65f}, {128, 128, 0.33f, 0.40f}, {64, 128, 0.19f, 0.22f}, {64, 64, 0.116f, 0.19f}};
+    int pick = 0;
+    float best = 0;
+    for (int i = 0; i < 5; ++i) {
+        const int64_t n = ((a.M + tiles[i].bm - 1) / tiles[i].bm) * ((a.N + tiles[i].bn - 1) / tiles[i].bn);
+        const float cost = fmaxf(tiles[i].alone, tiles[i].full * (float)((n + 255) / 256));
+        if (i == 0 || cost < best) { best = cost; pick = i; }
+    }
+    switch (pick) {
+        case 0: return launch_tile<AF, 2, 2, 4, 4, EXACT, ODT>(a, st);
+        case 1: return launch_tile<AF, 2, 2, 4, 3, EXACT, ODT>(a, st);
+        case 2: return launch_tile<AF, 2, 2, 2, 2, EXACT, ODT>(a, st);
+        case 3: return launch_tile<AF, 2, 2, 1, 2, EXACT, ODT>(a, st);
+        default: return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
+    }
 }
 
 static inline bool mx_side_ok(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int64_t rows, int64_t nb, int fmt) {
