@@ -11,10 +11,15 @@
 // relative error of a few 1e-6 of the result, which a 16-bit output's rounding (2e-3) hides.  For a 32-bit output the 8-bit operand is
 // split by the top bit of its exponent into two operands of 8 binades each, both exact, at twice the matrix work.
 #include <math.h>
+#include <atomic>
 #include "mx_common.h"
 #include "../../include/edadm.h"
+#ifndef MX_AF
+#error "compile with -DMX_AF=4|8"
+#endif
 
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
+typedef int mx_i4 __attribute__((ext_vector_type(4)));
 typedef float mx_f4 __attribute__((ext_vector_type(4)));
 
 struct MxArgs {
@@ -34,6 +39,8 @@ template <int N, typename F> __device__ __forceinline__ void mx_unroll(F&& f) {
         f(mx_int<N - 1>{});
     }
 }
+__device__ __forceinline__ mx_i8 frag4(mx_i4 a) { return mx_i8{a[0], a[1], a[2], a[3], 0, 0, 0, 0}; }
+__device__ __forceinline__ mx_i8 frag8(mx_i4 a, mx_i4 b) { return mx_i8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 __device__ __forceinline__ mx_i8 frag4(uint4 a) { return mx_i8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}; }
 __device__ __forceinline__ mx_i8 frag8(uint4 a, uint4 b) { return mx_i8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w}; }
 
@@ -99,7 +106,7 @@ typedef uint32_t mx_u64 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
 
 template <int AF, int MT, int NT> struct MxPair {                     // a lane's operands of two K-steps
-    uint4 w[NT][2], x[MT][AF == MX_FP4 ? 2 : 4];
+    mx_i4 w[NT][2], x[MT][AF == MX_FP4 ? 2 : 4];
     uint32_t sw[NT][2], sa[MT][2];
 };
 
@@ -112,6 +119,7 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
     const int r = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)(blockIdx.x % strips) * (16 * NT), m0 = (int64_t)(blockIdx.x / strips) * (16 * MT);
     const uint8_t *wp[NT], *wsp[NT], *ap[MT], *asp[MT];
+    bool here[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int64_t n = min(n0 + 16 * j + r, a.N - 1);              // rows past the end: read the last one, store nothing
@@ -123,6 +131,7 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
         const int64_t m = min(m0 + 16 * i + r, a.M - 1);
         ap[i] = a.A + m * a.lda;
         asp[i] = a.As + m * a.ldas;
+        here[i] = m0 + 16 * i + r < a.M;
     }
     // a whole pair: eight blocks; the 16-byte pieces of a lane are blocks q and 4 + q (4 bits), halves of blocks (8 bits)
     auto fetch = [&](int pair, MxPair<AF, MT, NT>& f) {
@@ -130,30 +139,33 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) f.w[j][u] = *(const uint4*)(wp[j] + b * 16 + u * 64 + q * 16);
+            for (int u = 0; u < 2; ++u) f.w[j][u] = *(const mx_i4*)(wp[j] + b * 16 + u * 64 + q * 16);
             const mx_u64 s = *(const mx_u64*)(wsp[j] + b);
             f.sw[j][0] = s[0];
             f.sw[j][1] = s[1];
         }
+        // lanes of rows that are not there load nothing (their old registers make rows that are not stored): one row of a costs the
+        // memory path a sixteenth of what a full tile does
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
+        for (int i = 0; i < MT; ++i)
+            if (here[i]) {
 #pragma unroll
-            for (int u = 0; u < NX; ++u) f.x[i][u] = *(const uint4*)(ap[i] + b * (NX * 8) + u * 64 + q * 16);
-            const mx_u64 s = *(const mx_u64*)(asp[i] + b);
-            f.sa[i][0] = s[0];
-            f.sa[i][1] = s[1];
-        }
+                for (int u = 0; u < NX; ++u) f.x[i][u] = *(const mx_i4*)(ap[i] + b * (NX * 8) + u * 64 + q * 16);
+                const mx_u64 s = *(const mx_u64*)(asp[i] + b);
+                f.sa[i][0] = s[0];
+                f.sa[i][1] = s[1];
+            }
     };
     // the last, short pair: blocks past the end are read from the last one and put to zero under a scale of 1
     auto fetch_end = [&](int pair, MxPair<AF, MT, NT>& f) {
         const int b = pair * 8, last = a.nblk - 1;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const mx_i4 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int k = b + 4 * u + q, kc = min(k, last);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const uint4 v = *(const uint4*)(wp[j] + (int64_t)kc * 16);
+                const mx_i4 v = *(const mx_i4*)(wp[j] + (int64_t)kc * 16);
                 const uint32_t s = wsp[j][kc];
                 f.w[j][u] = k <= last ? v : zero;
                 f.sw[j][u] = (k <= last ? s : 127u) << (8 * q);
@@ -169,7 +181,7 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
             const int k = AF == MX_FP4 ? b + 4 * u + q : b + 2 * u + (q >> 1), kc = min(k, last);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const uint4 v = *(const uint4*)(ap[i] + (AF == MX_FP4 ? (int64_t)kc * 16 : (int64_t)kc * 32 + (q & 1) * 16));
+                const mx_i4 v = *(const mx_i4*)(ap[i] + (AF == MX_FP4 ? (int64_t)kc * 16 : (int64_t)kc * 32 + (q & 1) * 16));
                 f.x[i][u] = k <= last ? v : zero;
             }
         }
@@ -193,7 +205,7 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
     const int whole = a.nblk / 8;
     int p = wave;
     if (p < whole) {
-        MxPair<AF, MT, NT> f[2];
+        MxPair<AF, MT, NT> f[2] = {};
         fetch(p, f[0]);
         while (true) {
             if (p + waves < whole) fetch(p + waves, f[1]);
@@ -252,9 +264,21 @@ __device__ __forceinline__ void mx_dma16(const void* base, uint32_t voff, uint32
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
 
+// the same, 4 bytes a lane
+__device__ __forceinline__ void mx_dma4(const void* base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
+}
+
 // everything in flight from memory has arrived (LDS: and from LDS); a form the compiler knows, so that it does not wait again for loads
 // that it would find behind newer ones
 template <bool LDS> __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(LDS ? 0x0070 : 0x0f70); }
+
+// index of this workgroup's tile: workgroups go round the 8 XCDs, so every XCD gets a run of neighbouring tiles, which share operands in
+// its L2
+__device__ __forceinline__ int mx_xcd_run(int total) {
+    const int each = total / 8, more = total % 8, x = (int)(blockIdx.x & 7);
+    return (x < more ? x * (each + 1) : more * (each + 1) + (x - more) * each) + (int)(blockIdx.x >> 3);
+}
 
 // a wave-uniform address in scalar registers
 __device__ __forceinline__ const void* mx_uniform(const void* p) {
@@ -274,6 +298,99 @@ __device__ __forceinline__ mx_f16v mx_mma32(mx_i8 w, mx_i8 a, mx_f16v c, uint32_
     }
 }
 
+// the blocks of K from `b` on, two at a time, straight into registers: rows m0 .. m0 + 32 MT - 1 by columns n0 .. n0 + 32 NT - 1
+template <int AF, int MT, int NT, bool EXACT>
+__device__ __forceinline__ void mx_rest(const MxArgs& a, int b, int64_t m0, int64_t n0, mx_f16v (&acc)[MT][NT]) {
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
+    for (; b < a.nblk; b += 2) {
+        const bool in = b + q < a.nblk;
+        const int k = in ? b + q : b, k1 = b + 1 < a.nblk ? b + 1 : b; // blocks past the end: read the last one, take zeros
+        const mx_i4 zero = {0, 0, 0, 0};
+        mx_i8 fx[MT], fw[NT];
+        uint32_t ta[MT], tw[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int64_t row = min(m0 + i * 32 + r, a.M - 1);
+            const uint8_t* p = a.A + row * a.lda;
+            if constexpr (AF == MX_FP4) {
+                const mx_i4 v = *(const mx_i4*)(p + (int64_t)k * 16);
+                fx[i] = frag4(in ? v : zero);
+            } else {
+                const mx_i4 v = *(const mx_i4*)(p + (int64_t)b * 32 + q * 16), v1 = *(const mx_i4*)(p + (int64_t)k1 * 32 + q * 16);
+                fx[i] = frag8(v, b + 1 < a.nblk ? v1 : zero);
+            }
+            const uint32_t t = a.As[row * a.ldas + k];
+            ta[i] = in ? t : 127u;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int64_t row = min(n0 + j * 32 + r, a.N - 1);
+            const mx_i4 v = *(const mx_i4*)(a.W + row * a.ldw + (int64_t)k * 16);
+            fw[j] = frag4(in ? v : zero);
+            const uint32_t t = a.Ws[row * a.ldws + k];
+            tw[j] = in ? t : 127u;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], tw[j], ta[i]);
+    }
+}
+
+// The wave's sums out through LDS (`mine`: its own part), 32 rows at a time: a lane holds four columns of one row, whole rows make whole
+// cache lines (stored straight from the registers this took 18 us a 256 x 256 tile, a fifth of the 5120-deep product).  Piece p (16 bytes)
+// of a row lies at p ^ turn(row), which spreads 16 rows over the banks.
+template <int NT, int ODT> struct MxOut {
+    static constexpr int SZ = ODT == MX_F32 ? 4 : 2, P = 32 * NT * SZ / 16, EL = 16 / SZ;   // pieces a row, elements a piece
+    static constexpr int PP = P > 16 ? 32 : P > 8 ? 16 : P > 4 ? 8 : 4;                     // a row's room in pieces
+    static constexpr int BYTES = 32 * PP * 16;
+};
+template <int MT, int NT, int ODT>
+__device__ __forceinline__ void mx_out_tile(const MxArgs& a, int64_t m0, int64_t n0, const mx_f16v (&acc)[MT][NT], uint8_t* mine) {
+    constexpr int SZ = MxOut<NT, ODT>::SZ, P = MxOut<NT, ODT>::P, PP = MxOut<NT, ODT>::PP, EL = MxOut<NT, ODT>::EL;
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
+    auto turn = [](int row) { return PP >= 16 ? row & 15 : (row / (16 / PP)) & (PP - 1); };
+    const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.ldo * SZ & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * j + 8 * g + 4 * q;                 // the wave's column
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+                if (a.bias) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += a.bias[min(n0 + c + e, a.N - 1)];
+                }
+                uint8_t* to = mine + r * (PP * 16) + ((c * SZ / 16) ^ turn(r)) * 16 + (c * SZ & 15);
+                if constexpr (ODT == MX_F32) *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
+                else *(uint2*)to = make_uint2(mx_pair<ODT>(v[0], v[1]), mx_pair<ODT>(v[2], v[3]));
+            }
+        const int64_t mw0 = m0 + i * 32;
+#pragma unroll
+        for (int k = 0; k < P / 2; ++k) {
+            const int row = (k * 64 + lane) / P, piece = (k * 64 + lane) % P;
+            const uint4 u = *(const uint4*)(mine + row * (PP * 16) + (piece ^ turn(row)) * 16);
+            const int64_t m = mw0 + row, n = n0 + piece * EL;
+            if (m >= a.M || n >= a.N) continue;
+            uint8_t* to = (uint8_t*)a.out + (m * a.ldo + n) * SZ;
+            if (wide && n + EL <= a.N) *(uint4*)to = u;
+            else {
+                const uint32_t d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < EL; ++e)
+                    if (n + e < a.N) {
+                        if constexpr (SZ == 4) ((uint32_t*)to)[e] = d[e];
+                        else ((uint16_t*)to)[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
+                    }
+            }
+        }
+    }
+}
+
 template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT>
 __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int tn) {
     constexpr int THREADS = 64 * WM * WN, BM = 32 * WM * MT, BN = 32 * WN * NT;
@@ -289,10 +406,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave / WN, wn = wave % WN;
 
-    // tile of this workgroup: workgroups go round the 8 XCDs, so every XCD gets a run of neighbouring tiles, walked eight tile rows
-    // at a time down the rows first: the tiles an XCD works on together share rows of a and of w in its L2
-    const int total = tm * tn, each = total / 8, more = total % 8, x = (int)(blockIdx.x & 7);
-    const int t = (x < more ? x * (each + 1) : more * (each + 1) + (x - more) * each) + (int)(blockIdx.x >> 3);
+    // the tiles of an XCD are walked eight tile rows at a time down the rows first: those it works on together share rows of a and of w
+    const int t = mx_xcd_run(tm * tn);
     const int band = t / (8 * tn), in = t - band * 8 * tn, high = min(8, tm - band * 8);
     // divided by the vector unit, uniform all the same
     const int ti = __builtin_amdgcn_readfirstlane(band * 8 + in % high), tj = __builtin_amdgcn_readfirstlane(in / high);
@@ -472,84 +587,98 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         if (s + 1 < steps) step(s++, mx_int<1>{}, mx_int<-1>{});
         step(s, mx_int<0>{}, mx_int<-1>{});
     }
-    for (int b = steps * STEP; b < a.nblk; b += 2) {                  // the rest of K, two blocks at a time
-        const bool in = b + q < a.nblk;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        mx_i8 fx[MT], fw[NT];
-        uint32_t ta[MT], tw[NT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int64_t row = min(m0 + (wm * MT + i) * 32 + r, a.M - 1);
-            const uint8_t* p = a.A + row * a.lda;
-            if constexpr (AF == MX_FP4) fx[i] = frag4(in ? *(const uint4*)(p + (int64_t)(b + q) * 16) : zero);
-            else fx[i] = frag8(*(const uint4*)(p + (int64_t)b * 32 + q * 16), b + 1 < a.nblk ? *(const uint4*)(p + (int64_t)b * 32 + 32 + q * 16) : zero);
-            ta[i] = in ? asb[aso[i] + b + q] : 127u;
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int64_t row = min(n0 + (wn * NT + j) * 32 + r, a.N - 1);
-            fw[j] = frag4(in ? *(const uint4*)(a.W + row * a.ldw + (int64_t)(b + q) * 16) : zero);
-            tw[j] = in ? wsb[wso[j] + b + q] : 127u;
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mma32<AF, EXACT, 0>(fw[j], fx[i], acc[i][j], tw[j], ta[i]);
-    }
-    // Out through LDS, 32 rows of the wave at a time: a lane holds four columns of one row, whole rows make whole cache lines (stored
-    // straight from the registers this took 18 us a tile, a fifth of the 5120-deep product).  Piece p (16 bytes) of a row lies at p ^ turn(row),
-    // which spreads 16 rows over the banks.
-    constexpr int SZ = ODT == MX_F32 ? 4 : 2, P = 32 * NT * SZ / 16, EL = 16 / SZ;     // pieces a row, elements a piece
-    constexpr int PP = P > 16 ? 32 : P > 8 ? 16 : P > 4 ? 8 : 4;                       // a row's room in pieces
-    auto turn = [](int row) { return PP >= 16 ? row & 15 : (row / (16 / PP)) & (PP - 1); };
-    static_assert(WM * WN * 32 * PP * 16 <= RING * STAGE, "");
-    uint8_t* mine = smem + wave * (32 * PP * 16);
-    const bool wide = ((uintptr_t)a.out & 15) == 0 && (a.ldo * SZ & 15) == 0;
-    const int64_t nw0 = n0 + wn * NT * 32;
+    mx_rest<AF, MT, NT, EXACT>(a, steps * STEP, m0 + wm * MT * 32, n0 + wn * NT * 32, acc);
+    static_assert(WM * WN * MxOut<NT, ODT>::BYTES <= RING * STAGE, "");
     __syncthreads();                                                  // every wave is done with the ring
+    mx_out_tile<MT, NT, ODT>(a, m0 + wm * MT * 32, n0 + wn * NT * 32, acc, smem + wave * MxOut<NT, ODT>::BYTES);
+}
+
+// ------------------------------------------------------------------------------------------------ a few dozen rows, or few tiles
+// At most a tile a CU and 8-bit a, where one step ahead does not hide the way to memory: 64 x 64 tiles, four waves of one 32 x 32
+// instruction each, steps of 128 elements through a ring of RING slots (an even number), RING - 2 of them in flight.  The scales lie in
+// the ring too (a dword a row and step), so that every wave issues the same PER loads a step and waits for the oldest steps by their count
+// alone; behind the last step that one is loaded again, to keep the count.  Needs scale rows on dword boundaries.
+#define MX_STREAM_RING 6
+#define MX_STREAM_LDS (MX_STREAM_RING * (64 * 128 + 64 * 64 + 512))
+template <bool EXACT, int ODT>
+__global__ __launch_bounds__(256) void k_mx_stream(MxArgs a, int tm) {
+    constexpr int AF = MX_FP8, AROW = 128, ABYTES = 64 * AROW, WBYTES = 64 * 64, STAGE = ABYTES + WBYTES + 512;
+    constexpr int RING = MX_STREAM_RING, AI = ABYTES / 4096, PER = AI + 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wm = wave >> 1, wn = wave & 1;
+    const int tile = mx_xcd_run(gridDim.x);
+    const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(tile % tm) * 64, n0 = (int64_t)__builtin_amdgcn_readfirstlane(tile / tm) * 64;
+    uint32_t av[AI], wv, sv;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int c = 32 * j + 8 * g + 4 * q;                 // the wave's column
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
-                if (a.bias) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += a.bias[min(nw0 + c + e, a.N - 1)];
-                }
-                uint8_t* to = mine + r * (PP * 16) + ((c * SZ / 16) ^ turn(r)) * 16 + (c * SZ & 15);
-                if constexpr (ODT == MX_F32) *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
-                else *(uint2*)to = make_uint2(mx_pair<ODT>(v[0], v[1]), mx_pair<ODT>(v[2], v[3]));
-            }
-        const int64_t mw0 = m0 + (wm * MT + i) * 32;
-#pragma unroll
-        for (int k = 0; k < P / 2; ++k) {
-            const int row = (k * 64 + lane) / P, piece = (k * 64 + lane) % P;
-            const uint4 u = *(const uint4*)(mine + row * (PP * 16) + (piece ^ turn(row)) * 16);
-            const int64_t m = mw0 + row, n = nw0 + piece * EL;
-            if (m >= a.M || n >= a.N) continue;
-            uint8_t* to = (uint8_t*)a.out + (m * a.ldo + n) * SZ;
-            if (wide && n + EL <= a.N) *(uint4*)to = u;
-            else {
-                const uint32_t d[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int e = 0; e < EL; ++e)
-                    if (n + e < a.N) {
-                        if constexpr (SZ == 4) ((uint32_t*)to)[e] = d[e];
-                        else ((uint16_t*)to)[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
-                    }
-            }
-        }
+    for (int i = 0; i < AI; ++i) {
+        const int row = (i * 256 + (int)threadIdx.x) / 8, p = (lane & 7) ^ ((row >> 1) & 7);
+        av[i] = (uint32_t)min((int64_t)row, a.M - 1 - m0) * (uint32_t)a.lda + p * 16;       // past the last row: read that one
     }
+    {
+        const int row = (int)threadIdx.x / 4, p = (lane & 3) ^ ((row >> 2) & 3);
+        wv = (uint32_t)min((int64_t)row, a.N - 1 - n0) * (uint32_t)a.ldw + p * 16;
+        sv = wn ? (uint32_t)min((int64_t)lane, a.N - 1 - n0) * (uint32_t)a.ldws : (uint32_t)min((int64_t)lane, a.M - 1 - m0) * (uint32_t)a.ldas;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const uint8_t *ab = a.A + m0 * a.lda, *wb = a.W + n0 * a.ldw, *sb = wn ? a.Ws + n0 * a.ldws : a.As + m0 * a.ldas;
+    auto load = [&](int step, int slot) {
+        const uint32_t la = lds0 + slot * STAGE;
+#pragma unroll
+        for (int i = 0; i < AI; ++i) mx_dma16(mx_uniform(ab + (int64_t)step * AROW), av[i], __builtin_amdgcn_readfirstlane(la + i * 4096 + wave * 1024));
+        mx_dma16(mx_uniform(wb + (int64_t)step * 64), wv, __builtin_amdgcn_readfirstlane(la + ABYTES + wave * 1024));
+        mx_dma4(mx_uniform(sb + (int64_t)step * 4), sv, __builtin_amdgcn_readfirstlane(la + ABYTES + WBYTES + wn * 256));   // both wm alike
+    };
+    mx_f16v acc[1][1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
+    // two steps at a time: the barrier, the way to LDS and back and the refill cost as much as the multiplications of both
+    const int steps = a.nblk / 4 & ~1;
+    if (steps) {
+        const int sx = (r >> 1) & 7, sz = (r >> 2) & 3;
+        const uint8_t *pa = smem + (wm * 32 + r) * AROW, *pw = smem + ABYTES + (wn * 32 + r) * 64, *ps = smem + ABYTES + WBYTES + r * 4;
+#pragma unroll
+        for (int d = 0; d < RING - 2; ++d) load(min(d, steps - 1), d);
+        int slot = 0, fill = RING - 2;
+        for (int s = 0; s < steps; s += 2) {
+            // (this wave's reads of the slots refilled below arrived before they were multiplied: the count says so to whoever moves code)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER * (RING - 4)) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            mx_i8 fx[2][2], fw[2][2];
+            uint32_t sa[2], sw[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = (slot + h) * STAGE;
+                sa[h] = *(const uint32_t*)(ps + at + wm * 128) >> (8 * q);
+                sw[h] = *(const uint32_t*)(ps + at + 256 + wn * 128) >> (8 * q);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    fw[h][t] = frag4(*(const mx_i4*)(pw + at + ((2 * t + q) ^ sz) * 16));
+                    fx[h][t] = frag8(*(const mx_i4*)(pa + at + ((4 * t + q) ^ sx) * 16), *(const mx_i4*)(pa + at + ((4 * t + 2 + q) ^ sx) * 16));
+                }
+            }
+            // the slots of the two steps before: every wave has multiplied what it read there
+            load(min(s + RING - 2, steps - 1), fill);
+            load(min(s + RING - 1, steps - 1), fill + 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                acc[0][0] = mx_mma32<AF, EXACT, 0>(fw[h][0], fx[h][0], acc[0][0], sw[h], sa[h]);
+                acc[0][0] = mx_mma32<AF, EXACT, 1>(fw[h][1], fx[h][1], acc[0][0], sw[h], sa[h]);
+            }
+            slot = slot + 2 == RING ? 0 : slot + 2;
+            fill = fill + 2 == RING ? 0 : fill + 2;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // the loads that kept the count
+    }
+    mx_rest<AF, 1, 1, EXACT>(a, steps * 4, m0 + wm * 32, n0 + wn * 32, acc);
+    __syncthreads();
+    mx_out_tile<1, 1, ODT>(a, m0 + wm * 32, n0 + wn * 32, acc, smem + wave * MxOut<1, ODT>::BYTES);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 template <int AF, int MT, int NT, bool EXACT, int ODT> static int launch_rows1(const MxArgs& a, hipStream_t st) {
-    constexpr int MAXW = MT * NT <= 2 ? 16 : 8;
+    constexpr int MAXW = 8;
     const int64_t strips = (a.N + 16 * NT - 1) / (16 * NT), chunks = (a.M + 16 * MT - 1) / (16 * MT);
     if (strips > 0x7fffffff || chunks > 0x7fffffff || strips * chunks > 0x7fffffff) return EDADM_EINVAL;
     // waves: two pairs each (one is fetched while the other multiplies) as far as they go
@@ -559,13 +688,25 @@ template <int AF, int MT, int NT, bool EXACT, int ODT> static int launch_rows1(c
     return edadm_launch_status();
 }
 template <int AF, bool EXACT, int ODT> static int launch_rows(const MxArgs& a, hipStream_t st) {
-    // rows of a are read by every strip of columns: the strip is as wide as the rows are many, as long as there are strips for the CUs
-    const int mt = (int)((a.M + 15) / 16);
-    const bool many = a.N >= 64 * 96;
-    if (mt == 1) return launch_rows1<AF, 1, 1, EXACT, ODT>(a, st);
-    if (mt == 2) return launch_rows1<AF, 2, 2, EXACT, ODT>(a, st);
-    if (mt == 3) return many ? launch_rows1<AF, 3, 4, EXACT, ODT>(a, st) : launch_rows1<AF, 3, 2, EXACT, ODT>(a, st);
-    return many ? launch_rows1<AF, 4, 4, EXACT, ODT>(a, st) : launch_rows1<AF, 4, 2, EXACT, ODT>(a, st);
+    // Every strip of columns reads all rows of a: strips are wide where rows are many, as long as that leaves 128 of them.  10240 x 10240:
+    // 16 rows 20 us on 64 columns, 25 on 32, 27 on 16; one row 16.4 us on 16 columns, 17.8 on 32; 32 rows 23 us on 48 columns, 35 on
+    // 32.  5120 x 5120: 16 rows 8.1 us on 32 columns, 10.1 on 16, 10.7 on 64.
+    if (a.M <= 2) return launch_rows1<AF, 1, 1, EXACT, ODT>(a, st);
+    if (a.M <= 16) return a.N >= 8192 ? launch_rows1<AF, 1, 4, EXACT, ODT>(a, st) : a.N >= 4096 ? launch_rows1<AF, 1, 2, EXACT, ODT>(a, st) : launch_rows1<AF, 1, 1, EXACT, ODT>(a, st);
+    return a.N >= 8192 ? launch_rows1<AF, 2, 3, EXACT, ODT>(a, st) : launch_rows1<AF, 2, 2, EXACT, ODT>(a, st);
+}
+
+// more LDS than a kernel gets by itself has to be asked for, once per kernel and device (asking again is harmless)
+template <int LDS> static int mx_room(const void* kernel) {
+    if (LDS <= 65536) return 0;
+    static std::atomic<const void*> done[EDADM_MAX_DEVICES][64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= EDADM_MAX_DEVICES) return EDADM_EIO;
+    std::atomic<const void*>* slot = &done[dev][((uintptr_t)kernel >> 4) % 64];
+    if (slot->load(std::memory_order_relaxed) == kernel) return 0;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return EDADM_EIO;
+    slot->store(kernel, std::memory_order_relaxed);
+    return 0;
 }
 
 template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static int launch_tile(const MxArgs& a, hipStream_t st) {
@@ -574,16 +715,7 @@ template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static in
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
     if (tm > 0x7fffffff / 8 || tn > 0x7fffffff / 8 || tm * tn > 0x7fffffff / 8) return EDADM_EINVAL;
     auto* k = &k_mx_tile<AF, WM, WN, MT, NT, EXACT, ODT>;
-    if (LDS > 65536) {
-        // once per kernel and device; setting it again is harmless
-        static bool done[EDADM_MAX_DEVICES] = {};
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= EDADM_MAX_DEVICES) return EDADM_EIO;
-        if (!done[dev]) {
-            if (hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return EDADM_EIO;
-            done[dev] = true;
-        }
-    }
+    if (int rc = mx_room<LDS>((const void*)k)) return rc;
     k<<<(unsigned)(tm * tn), 64 * WM * WN, LDS, st>>>(a, (int)tm, (int)tn);
     return edadm_launch_status();
 }
@@ -591,7 +723,7 @@ template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static in
 template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hipStream_t st) {
     // the tiled kernel's 32-bit row offsets: 256 rows of a and of w under 4 GB
     const bool fits = a.lda < (1 << 23) && a.ldw < (1 << 23) && a.ldas < (1 << 23) && a.ldws < (1 << 23);
-    if (a.M <= 64 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
+    if (a.M <= 32 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
     // The tile is the one of least cost: tiles a CU x what a tile costs on a full chip, and no less than what one costs alone (both
     // in units of a 256 x 256 tile on a full chip, 68 us at K = 5120 with 8-bit a, 44 us with 4-bit a; measured over M = 64 .. 8192,
     // the ratios are the same for both).  4096 x 5120 x 5120: 256 x 256 leaves three quarters of the second round empty (81 us, 4-bit
@@ -610,9 +742,30 @@ template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hip
         case 1: return launch_tile<AF, 2, 2, 4, 3, EXACT, ODT>(a, st);
         case 2: return launch_tile<AF, 2, 2, 2, 2, EXACT, ODT>(a, st);
         case 3: return launch_tile<AF, 2, 2, 1, 2, EXACT, ODT>(a, st);
-        default: return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
+        default: break;
     }
+    // 8-bit a, at most one 64 x 64 tile a CU: the deep ring (48 x 10240 x 5120 12.8 against 15.6 us, 64 x 10240 x 10240 31 against 41);
+    // more of them: four of the plain ring's workgroups fit a CU and hide each other's waits (256 x 5120 x 5120 16.3 against 22.2).  4-bit
+    // a: the plain ring's steps are twice as long (64 x 5120 x 5120 8.7 us against 10.6 in steps of 128)
+    if constexpr (AF == MX_FP8) {
+        const int64_t tiles64 = ((a.M + 63) / 64) * ((a.N + 63) / 64);
+        if (tiles64 <= 256 && (((uintptr_t)a.As | (uintptr_t)a.Ws | (uintptr_t)a.ldas | (uintptr_t)a.ldws) & 3) == 0) {
+            auto* k = &k_mx_stream<EXACT, ODT>;
+            if (int rc = mx_room<MX_STREAM_LDS>((const void*)k)) return rc;
+            k<<<(unsigned)tiles64, 256, MX_STREAM_LDS, st>>>(a, (int)((a.M + 63) / 64));
+            return edadm_launch_status();
+        }
+    }
+    return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
 }
+
+// one object per type of a (they build in parallel); the entry point stands in the 8-bit one
+#if MX_AF == MX_FP4
+int mx_gemm_a4(const MxArgs& a, int odt, hipStream_t st) {
+    return odt == MX_F32 ? launch_mx<MX_FP4, false, MX_F32>(a, st) : odt == MX_BF16 ? launch_mx<MX_FP4, false, MX_BF16>(a, st) : launch_mx<MX_FP4, false, MX_F16>(a, st);
+}
+#else
+int mx_gemm_a4(const MxArgs& a, int odt, hipStream_t st);
 
 static inline bool mx_side_ok(const uint8_t* c, int64_t ld, const uint8_t* s, int64_t lds, int64_t rows, int64_t nb, int fmt) {
     return c && s && (uintptr_t)c % 16 == 0 && ld >= nb * (fmt == MX_FP4 ? 16 : 32) && (rows <= 1 || ld % 16 == 0) && lds >= nb;
@@ -627,7 +780,7 @@ extern "C" int edadm_mx_gemm(const uint8_t* A, int64_t lda, const uint8_t* As, i
     if (!mx_side_ok(A, lda, As, ldas, M, nb, afmt) || !mx_side_ok(W, ldw, Ws, ldws, N, nb, MX_FP4) || !out || ldo < N) return EDADM_EINVAL;
     const MxArgs a = {A, As, W, Ws, lda, ldas, ldw, ldws, bias, out, ldo, M, N, (int)nb};
     hipStream_t st = (hipStream_t)stream;
-    if (afmt == MX_FP4)
-        return odt == MX_F32 ? launch_mx<MX_FP4, false, MX_F32>(a, st) : odt == MX_BF16 ? launch_mx<MX_FP4, false, MX_BF16>(a, st) : launch_mx<MX_FP4, false, MX_F16>(a, st);
+    if (afmt == MX_FP4) return mx_gemm_a4(a, odt, st);
     return odt == MX_F32 ? launch_mx<MX_FP8, true, MX_F32>(a, st) : odt == MX_BF16 ? launch_mx<MX_FP8, false, MX_BF16>(a, st) : launch_mx<MX_FP8, false, MX_F16>(a, st);
 }
+#endif

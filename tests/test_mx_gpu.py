@@ -47,6 +47,20 @@ def check_codes(q, x2d, fmt):
     return code, byte
 
 
+def test_first_calls_inside_a_capture(ops):
+    """the first call of a kernel that asks for more LDS than it gets by itself, made while a graph is captured (this test stands first)"""
+    for m, n in ((2048, 5120), (40, 128)):
+        a, w = ops.mx_quantize(torch.randn(m, 512, device="cuda"), "mxfp8"), ops.mx_quantize(torch.randn(n, 512, device="cuda"), "mxfp4")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.mx_gemm(a, w, dtype=torch.float16)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ops.mx_gemm(a, w, dtype=torch.float16))
+
+
 # ------------------------------------------------------------------------------------------------ quantisation and its inverse
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -325,7 +339,7 @@ def check_product(got, va, vw, bias, dtype, fmt):
     ref = va @ vw.t() + (0 if bias is None else bias.double())
     size = va.abs() @ vw.abs().t() + (0 if bias is None else bias.double().abs())
     tol = (k / 16 + 16) * 2.0 ** -23 * size
-    got = got.cpu().double()
+    got = got.to(va.device).double()
     if dtype != torch.float32:
         tol = tol + HALF[dtype] * ref.abs() * 1.001 + (2.0 ** -25 if dtype == torch.float16 else 0) + (2.0 ** -13 * size if fmt == "mxfp8" else 0)
         assert float((got - ref).norm()) <= (HALF[dtype] + 1e-4) * float(ref.norm()) + 1e-6
@@ -349,6 +363,38 @@ def test_product(ops, mnk, fmt):
         got = ops.mx_gemm(a, w, bias=bias.cuda(), dtype=dtype)
         check_product(got, va, vw, bias, dtype, fmt)
         same(ops.mx_gemm(a, w, bias=bias.cuda(), dtype=dtype), got)      # the same bits again
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("k", [64, 160, 288, 544, 1000, 1056, 1280, 1504, 2592])
+@pytest.mark.parametrize("mn", [(4096, 4096), (4000, 4090), (2048, 5120), (1900, 5001), (2560, 2560), (2500, 2501), (1024, 2560), (1000, 2500), (100, 200), (64, 640)])
+def test_product_tiles(ops, mn, k, fmt):
+    """every tile of the product (256 x 256, 256 x 192, 128 x 128, 64 x 128, 64 x 64) with whole and cut edges, over K with no, one, an
+    odd and an even number of whole steps, with and without a short end, scale rows on and off dword boundaries"""
+    m, n = mn
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    a = ops.mx_quantize(torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(k, generator=g, device="cuda")), fmt)
+    w = ops.mx_quantize(torch.randn(n, k, generator=g, device="cuda") * 0.02, "mxfp4")
+    va, vw = ops.mx_dequantize(a).double(), ops.mx_dequantize(w).double()
+    bias = torch.randn(n, generator=g, device="cuda")
+    for dtype in DTYPES:
+        got = ops.mx_gemm(a, w, bias=bias, dtype=dtype)
+        check_product(got, va, vw, bias, dtype, fmt)
+        assert torch.equal(ops.mx_gemm(a, w, bias=bias, dtype=dtype), got)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 16, 17, 32, 33])
+@pytest.mark.parametrize("n", [64, 4100, 8200])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_product_few_rows(ops, m, n, fmt):
+    """the few-row kernel's widths of strip, K from one block to more pairs of steps than its waves hold"""
+    for k in (31, 128, 256, 480, 5000):
+        g = torch.Generator("cuda").manual_seed(m + n + k)
+        a = ops.mx_quantize(torch.randn(m, k, generator=g, device="cuda"), fmt)
+        w = ops.mx_quantize(torch.randn(n, k, generator=g, device="cuda"), "mxfp4")
+        va, vw = ops.mx_dequantize(a).double(), ops.mx_dequantize(w).double()
+        for dtype in (torch.float32, torch.bfloat16):
+            check_product(ops.mx_gemm(a, w, dtype=dtype), va, vw, None, dtype, fmt)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
