@@ -12,82 +12,61 @@ enum { MX_QUANT = 0, MX_FAKE = 1, MX_GRAD = 2 };
 
 // ------------------------------------------------------------------------------------------------ element-wise forms
 // An item is 8 elements of a row; a row has `items` = 4 x blocks of them.  Dense tensors with whole blocks come as ONE row (the
-// host folds them), so the row index is only divided out for ragged or strided rows.  U items per thread, a block's width apart,
-// all loads issued before the first use.
-template <int DT, int FMT, int OP, bool VEC, int U>
+// host folds them), so the row index is only divided out for ragged or strided rows.  One item a thread: two or four of them, a
+// workgroup's width apart, made no form faster and the 16-bit ones slower (10240 x 5120 bf16 to e4m3: 30.3 us, 5.25 TB/s with one, 32.8
+// with four; fp32 to e2m1 40.0 and 41.3; fake quantisation bf16 34.2, 6.1 TB/s, and 37.4): the waves are enough loads in flight.
+__device__ __forceinline__ void mx_place(int64_t i, int64_t total, int64_t rows, int64_t items, int64_t& row, int64_t& it) {
+    if (rows == 1) { row = 0; it = i; }
+    else if (total <= 0x7fffffff) { row = (uint32_t)i / (uint32_t)items; it = (uint32_t)i - (uint32_t)row * (uint32_t)items; }
+    else { row = i / items; it = i - row * items; }
+}
+
+template <int DT, int FMT, int OP, bool VEC>
 __global__ __launch_bounds__(256) void k_mx_elem(const void* __restrict__ x, int64_t ldx, const void* __restrict__ gy, int64_t ldg,
                                                  void* __restrict__ out, int64_t ldo, uint8_t* __restrict__ codes, int64_t ldc,
                                                  uint8_t* __restrict__ scales, int64_t lds, int64_t rows, int64_t cols, int64_t items) {
-    const int64_t total = rows * items, first = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
-    float v[U][8], g[U][8];
-    int64_t row[U], it[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t i = first + u * 256;
-        if (rows == 1) { row[u] = 0; it[u] = i; }
-        else if (total <= 0x7fffffff) { row[u] = (uint32_t)i / (uint32_t)items; it[u] = (uint32_t)i - (uint32_t)row[u] * (uint32_t)items; }
-        else { row[u] = i / items; it[u] = i - row[u] * items; }
-        const int64_t left = cols - it[u] * 8;
-        const int valid = i < total ? (int)(left < 8 ? left : 8) : 0;
-        if (valid > 0) {
-            mx_load8<DT, VEC>(x, row[u] * ldx + it[u] * 8, valid, v[u]);
-            if constexpr (OP == MX_GRAD) mx_load8<DT, VEC>(gy, row[u] * ldg + it[u] * 8, valid, g[u]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { v[u][e] = 0.f; if constexpr (OP == MX_GRAD) g[u][e] = 0.f; }
-        }
+    const int64_t total = rows * items, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;                                           // whole quads: items is a multiple of 4
+    int64_t row, it;
+    mx_place(i, total, rows, items, row, it);
+    const int64_t left = cols - it * 8;
+    const int valid = (int)(left < 8 ? left : 8);
+    float v[8] = {}, g[8] = {};
+    if (valid > 0) {
+        mx_load8<DT, VEC>(x, row * ldx + it * 8, valid, v);
+        if constexpr (OP == MX_GRAD) mx_load8<DT, VEC>(gy, row * ldg + it * 8, valid, g);
     }
+    if constexpr (OP == MX_QUANT) {
+        const uint32_t b = mx_block_exp<FMT>(v);
+        mx_put<FMT>(codes + row * ldc, scales + row * lds, it, mx_encode8<FMT>(v, b, mx_scale(b)), b);
+    } else if constexpr (OP == MX_FAKE) {
+        mx_fake8<FMT>(v);
+        if (valid > 0) mx_store8<DT, VEC>(out, row * ldo + it * 8, valid, v);
+    } else {
+        const float top = mx_top<FMT>(v);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (first + u * 256 >= total) break;                          // whole quads: items is a multiple of 4
-        const int64_t left = cols - it[u] * 8;
-        const int valid = (int)(left < 8 ? left : 8);
-        if constexpr (OP == MX_QUANT) {
-            const uint32_t b = mx_block_exp<FMT>(v[u]);
-            mx_put<FMT>(codes + row[u] * ldc, scales + row[u] * lds, it[u], mx_encode8<FMT>(v[u], b, mx_scale(b)), b);
-        } else if constexpr (OP == MX_FAKE) {
-            mx_fake8<FMT>(v[u]);
-            if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, v[u]);
-        } else {
-            const float top = mx_top<FMT>(v[u]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[u][e] = fabsf(v[u][e]) <= top ? g[u][e] : 0.f;
-            if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, g[u]);
-        }
+        for (int e = 0; e < 8; ++e) g[e] = fabsf(v[e]) <= top ? g[e] : 0.f;
+        if (valid > 0) mx_store8<DT, VEC>(out, row * ldo + it * 8, valid, g);
     }
 }
 
-template <int DT, int FMT, bool VEC, int U>
+template <int DT, int FMT, bool VEC>
 __global__ __launch_bounds__(256) void k_mx_read(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
                                                  int64_t lds, void* __restrict__ out, int64_t ldo, int64_t rows, int64_t cols,
                                                  int64_t items) {
-    const int64_t total = rows * items, first = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
-    uint2 c[U];
-    uint32_t b[U];
-    int64_t row[U], it[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t i = first + u * 256;
-        if (rows == 1) { row[u] = 0; it[u] = i; }
-        else if (total <= 0x7fffffff) { row[u] = (uint32_t)i / (uint32_t)items; it[u] = (uint32_t)i - (uint32_t)row[u] * (uint32_t)items; }
-        else { row[u] = i / items; it[u] = i - row[u] * items; }
-        c[u] = make_uint2(0, 0);
-        b[u] = 0;
-        if (i < total) {
-            if constexpr (FMT == MX_FP4) c[u].x = *(const uint32_t*)(codes + row[u] * ldc + it[u] * 4);
-            else c[u] = *(const uint2*)(codes + row[u] * ldc + it[u] * 8);
-            b[u] = scales[row[u] * lds + (it[u] >> 2)];
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (first + u * 256 >= total) break;
-        const int64_t left = cols - it[u] * 8;
-        const int valid = (int)(left < 8 ? left : 8);
-        float v[8];
-        mx_decode8<FMT>(c[u], mx_scale(b[u]), v);
-        if (valid > 0) mx_store8<DT, VEC>(out, row[u] * ldo + it[u] * 8, valid, v);
-    }
+    const int64_t total = rows * items, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    int64_t row, it;
+    mx_place(i, total, rows, items, row, it);
+    const int64_t left = cols - it * 8;
+    const int valid = (int)(left < 8 ? left : 8);
+    if (valid <= 0) return;
+    uint2 c = make_uint2(0, 0);
+    if constexpr (FMT == MX_FP4) c.x = *(const uint32_t*)(codes + row * ldc + it * 4);
+    else c = *(const uint2*)(codes + row * ldc + it * 8);
+    float v[8];
+    mx_decode8<FMT>(c, mx_scale(scales[row * lds + (it >> 2)]), v);
+    mx_store8<DT, VEC>(out, row * ldo + it * 8, valid, v);
 }
 
 // ------------------------------------------------------------------------------------------------ root-mean-square norm
@@ -178,11 +157,12 @@ __global__ __launch_bounds__(1024) void k_rmsnorm(const void* __restrict__ x, in
 
 // Backward.  With g the output's gradient where the element was inside its block's range (0 elsewhere), xh = h rstd:
 //   dh = gh + rstd (g w - xh mean(g w xh)),   dw = sum over rows g xh.
-// The range is found again from h, rstd and w (no mask is kept).  Rows of up to two eights a thread keep w and gh in registers too;
-// four eights would not fit beside them, and read those where they are used.  A workgroup walks rows blockIdx, blockIdx + grid, ...; its share of
-// dw stays in registers and goes out once, as a row of `part`, which k_colsum adds up in a fixed order in 64 bits.
-template <int DT, bool WF32, int VPT, bool VEC>
-__global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ gy, int64_t ldg, const void* __restrict__ gh,
+// The range is found again from h, rstd and w (no mask is kept).  A workgroup walks rows blockIdx, blockIdx + grid, ..., the next row
+// on its way from memory while the current one is reduced; its share of dw stays in registers and goes out once, as a row of `part`,
+// which k_colsum adds up in a fixed order in 64 bits.  Rows of up to two eights a thread keep w in registers too; four eights would not
+// fit beside the rest, and read it where it is used.
+template <int DT, bool WF32, int VPT, bool VEC, int MAXT>
+__global__ __launch_bounds__(MAXT) void k_rmsnorm_bwd(const void* __restrict__ gy, int64_t ldg, const void* __restrict__ gh,
                                                       int64_t ldgh, const void* __restrict__ h, int64_t ldh,
                                                       const float* __restrict__ rstd, const void* __restrict__ w,
                                                       void* __restrict__ dh, int64_t ldd, float* __restrict__ part, int64_t rows,
@@ -192,9 +172,12 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ g
     constexpr int WDT = WF32 ? MX_F32 : DT;
     constexpr bool HOLD = VPT <= 2;
     float wh[HOLD ? VPT : 1][8], acc[VPT][8];
-    auto load_w = [&](int k, float (&wv)[8]) {
+    auto valid_of = [&](int k) {
         const int64_t left = cols - (int64_t)(t + k * tpr) * 8;
-        const int valid = (int)(left < 8 ? left : 8);
+        return (int)(left < 8 ? left : 8);
+    };
+    auto load_w = [&](int k, float (&wv)[8]) {
+        const int valid = valid_of(k);
 #pragma unroll
         for (int e = 0; e < 8; ++e) wv[e] = 0.f;
         if (valid > 0) mx_load8<WDT, VEC>(w, (int64_t)(t + k * tpr) * 8, valid, wv);
@@ -205,24 +188,35 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ g
         for (int e = 0; e < 8; ++e) acc[k][e] = 0.f;
         if constexpr (HOLD) load_w(k, wh[k]);
     }
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * slots + slot; row < rows; row += (int64_t)gridDim.x * slots, turn ^= 1) {
-        const float rs = rstd[row];
-        float g[VPT][8], xh[VPT][8], uh[HOLD ? VPT : 1][8];
-        double dot = 0;
+    mx_raw<DT, VEC> rh[VPT] = {}, rg[VPT] = {}, ru[VPT] = {};         // eights past the row's end stay zero
+    float rs_next = 0.f;
+    auto fetch = [&](int64_t row) {
+        rs_next = rstd[row];
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int it = t + k * tpr;
-            const int64_t left = cols - (int64_t)it * 8;
-            const int valid = (int)(left < 8 ? left : 8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { g[k][e] = 0.f; xh[k][e] = 0.f; if constexpr (HOLD) uh[k][e] = 0.f; }
+            const int valid = valid_of(k);
             if (valid > 0) {
-                mx_load8<DT, VEC>(h, row * ldh + it * 8, valid, xh[k]);
-                mx_load8<DT, VEC>(gy, row * ldg + it * 8, valid, g[k]);
-                if constexpr (HOLD) if (gh) mx_load8<DT, VEC>(gh, row * ldgh + it * 8, valid, uh[k]);
+                const int64_t at = (int64_t)(t + k * tpr) * 8;
+                mx_fetch8<DT, VEC>(h, row * ldh + at, valid, rh[k]);
+                mx_fetch8<DT, VEC>(gy, row * ldg + at, valid, rg[k]);
+                if (gh) mx_fetch8<DT, VEC>(gh, row * ldgh + at, valid, ru[k]);
             }
         }
+    };
+    const int64_t stride = (int64_t)gridDim.x * slots;
+    int64_t row = (int64_t)blockIdx.x * slots + slot;
+    if (row < rows) fetch(row);
+    for (int turn = 0; row < rows; row += stride, turn ^= 1) {
+        const float rs = rs_next;
+        float g[VPT][8], xh[VPT][8], up[VPT][8];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            mx_unpack8<DT, VEC>(rh[k], xh[k]);
+            mx_unpack8<DT, VEC>(rg[k], g[k]);
+            mx_unpack8<DT, VEC>(ru[k], up[k]);
+        }
+        if (row + stride < rows) fetch(row + stride);
+        double dot = 0;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int it = t + k * tpr;
@@ -236,7 +230,7 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ g
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 xh[k][e] *= rs;
-                y[e] = e < left ? xh[k][e] * wv[e] : 0.f;          // the forward's rounding
+                y[e] = e < left ? xh[k][e] * wv[e] : 0.f;             // the forward's rounding
             }
             if (fmt) {
                 const float top = fmt == MX_FP4 ? mx_top<MX_FP4>(y) : mx_top<MX_FP8>(y);
@@ -252,21 +246,15 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ g
             }
             dot += s;
         }
-        // the two slots of sm alternate, so that one barrier a row is enough: a wave is at most one row ahead
+        // the two halves of sm alternate, so that one barrier a row is enough: a wave is at most one row ahead
         const float mean = (float)(row_sum(dot, tpr, sm[turn]) / (double)cols);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int it = t + k * tpr;
-            const int64_t left = cols - (int64_t)it * 8;
-            const int valid = (int)(left < 8 ? left : 8);
+            const int valid = valid_of(k);
             if (valid > 0) {
-                float up[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) up[e] = HOLD ? uh[HOLD ? k : 0][e] : 0.f;
-                if constexpr (!HOLD) if (gh) mx_load8<DT, VEC>(gh, row * ldgh + it * 8, valid, up);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) up[e] = fmaf(rs, fmaf(-mean, xh[k][e], g[k][e]), up[e]);
-                mx_store8<DT, VEC>(dh, row * ldd + it * 8, valid, up);
+                for (int e = 0; e < 8; ++e) up[k][e] = fmaf(rs, fmaf(-mean, xh[k][e], g[k][e]), up[k][e]);
+                mx_store8<DT, VEC>(dh, row * ldd + (int64_t)(t + k * tpr) * 8, valid, up[k]);
             }
         }
     }
@@ -278,18 +266,31 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_bwd(const void* __restrict__ g
     }
 }
 
-// dw[c] = sum over n rows of part[.][ld], 32 columns to a workgroup, 32 lanes down each column, added in a fixed order
+// dw[c] = sum over n rows of part[.][ld], 16 columns to a workgroup, 64 lanes down each column, added in a fixed order
 template <int WDT> __global__ __launch_bounds__(1024) void k_colsum(const float* __restrict__ part, int64_t ld, int n, void* __restrict__ dw, int64_t cols) {
-    __shared__ double sm[32][33];
-    const int c = threadIdx.x & 31, p = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    __shared__ double sm[64][17];
+    const int c = threadIdx.x & 15, p = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c;
     double s = 0;
-    if (col < cols)
-        for (int i = p; i < n; i += 32) s += (double)part[(int64_t)i * ld + col];
+    if (col < cols) {
+        int i = p;
+        for (; i + 192 < n; i += 256) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = part[(int64_t)(i + 64 * k) * ld + col];
+            s += ((double)v[0] + (double)v[1]) + ((double)v[2] + (double)v[3]);
+        }
+        for (; i < n; i += 64) s += (double)part[(int64_t)i * ld + col];
+    }
     sm[p][c] = s;
     __syncthreads();
+    if (p < 4) {                                                      // four lanes a column, then one
+        for (int i = p + 4; i < 64; i += 4) s += sm[i][c];
+        sm[p][c] = s;
+    }
+    __syncthreads();
     if (p == 0 && col < cols) {
-        for (int i = 1; i < 32; ++i) s += sm[i][c];
+        s = (sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]);
         if constexpr (WDT == MX_F32) ((float*)dw)[col] = (float)s;
         else ((uint16_t*)dw)[col] = (uint16_t)mx_pair<WDT>((float)s, 0.f);
     }
@@ -322,20 +323,17 @@ static int mx_elem(const void* x, int64_t ldx, const void* gy, int64_t ldg, int 
         rows = 1;
     }
     const int64_t items = mx_blocks(cols) * 4, total = rows * items;
-    // work per thread: one item where more would leave the 256 CUs without eight waves each, else 64 bytes of x in flight
-    const bool wide = total >= (int64_t)256 * 8 * 64 * 4;
     hipStream_t st = (hipStream_t)stream;
-#define MX_GO(V, U)                                                                                                              \
+#define MX_GO(V)                                                                                                                 \
     do {                                                                                                                         \
-        const int64_t grid = (total + 256 * U - 1) / (256 * U);                                                                  \
+        const int64_t grid = (total + 255) / 256;                                                                                \
         if (grid > 0x7fffffff) return EDADM_EINVAL;                                                                              \
-        if (fmt == MX_FP4) k_mx_elem<DT, MX_FP4, OP, V, U><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
-        else k_mx_elem<DT, MX_FP8, OP, V, U><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
+        if (fmt == MX_FP4) k_mx_elem<DT, MX_FP4, OP, V><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
+        else k_mx_elem<DT, MX_FP8, OP, V><<<(unsigned)grid, 256, 0, st>>>(x, ldx, gy, ldg, out, ldo, codes, ldc, scales, lds, rows, cols, items); \
     } while (0)
     MX_DT(dt, {
-        if (!vec) MX_GO(false, 1);
-        else if (wide) MX_GO(true, (DT == MX_F32 ? 2 : 4));
-        else MX_GO(true, 1);
+        if (vec) MX_GO(true);
+        else MX_GO(false);
     })
 #undef MX_GO
     return edadm_launch_status();
@@ -381,19 +379,17 @@ extern "C" int edadm_mx_dequantize(const uint8_t* codes, int64_t ldc, const uint
         rows = 1;
     }
     const int64_t items = mx_blocks(cols) * 4, total = rows * items;
-    const bool wide = total >= (int64_t)256 * 8 * 64 * 4;
     hipStream_t st = (hipStream_t)stream;
-#define MX_GO(V, U)                                                                                                              \
+#define MX_GO(V)                                                                                                                 \
     do {                                                                                                                         \
-        const int64_t grid = (total + 256 * U - 1) / (256 * U);                                                                  \
+        const int64_t grid = (total + 255) / 256;                                                                                \
         if (grid > 0x7fffffff) return EDADM_EINVAL;                                                                              \
-        if (fmt == MX_FP4) k_mx_read<DT, MX_FP4, V, U><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items); \
-        else k_mx_read<DT, MX_FP8, V, U><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items);   \
+        if (fmt == MX_FP4) k_mx_read<DT, MX_FP4, V><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items); \
+        else k_mx_read<DT, MX_FP8, V><<<(unsigned)grid, 256, 0, st>>>(codes, ldc, scales, lds, out, ldo, rows, cols, items);   \
     } while (0)
     MX_DT(dt, {
-        if (!vec) MX_GO(false, 1);
-        else if (wide) MX_GO(true, (DT == MX_F32 ? 2 : 4));
-        else MX_GO(true, 1);
+        if (vec) MX_GO(true);
+        else MX_GO(false);
     })
 #undef MX_GO
     return edadm_launch_status();
@@ -401,8 +397,8 @@ extern "C" int edadm_mx_dequantize(const uint8_t* codes, int64_t ldc, const uint
 
 #define RMS_MAX_COLS 32768      // 1024 threads x 4 eights
 
-// threads per row and eights per thread: the fewest eights that keep a row within 1024 threads, more of them where there are
-// rows enough to fill the chip anyway (fewer waves, more loads in flight in each)
+// threads per row and eights per thread: one wave a row where many short rows fill the chip; else two eights a thread where rows are
+// many (10240 x 5120: 76.8 us, 4.8 TB/s; one eight 95.8, four 79.4), one where they are few, more where 1024 threads demand it
 static inline void rms_shape(int64_t rows, int64_t items, int* vpt, int* tpr) {
     int v = rows >= 2048 ? 2 : 1;
     if (items <= 64 * 4 && rows >= 2048) v = items <= 64 ? 1 : items <= 128 ? 2 : 4;
@@ -434,23 +430,36 @@ extern "C" int edadm_rmsnorm_fwd(const void* x, int64_t ldx, const void* res, in
 #define RMS_V(W, V) do { if (vpt == 1) RMS_GO(W, 1, V); else if (vpt == 2) RMS_GO(W, 2, V); else RMS_GO(W, 4, V); } while (0)
     MX_DT(dt, {
         if (weight_f32 || dt == MX_F32) { if (vec) RMS_V(true, true); else RMS_V(true, false); }
-        else { if (vec) RMS_V(false, true); else RMS_V(false, false); }
+        else if constexpr (DT != MX_F32) { if (vec) RMS_V(false, true); else RMS_V(false, false); }
     })
 #undef RMS_V
 #undef RMS_GO
     return edadm_launch_status();
 }
 
-// rows of `part`: as many workgroups as the chip holds at once, four row slots each where a row is one wave
+// the backward's: the same for short rows, else the fewest eights that 512 threads hold, which keep its state without spilling up to
+// 16384 columns (4096 x 2560: one eight 23.5 us, two 26.4, four 36.6)
+static inline void rms_bwd_shape(int64_t rows, int64_t items, int* vpt, int* tpr) {
+    rms_shape(rows, items, vpt, tpr);
+    if (*tpr == 64) return;
+    int v = 1;
+    while ((items + v - 1) / v > 512 && v < 4) v *= 2;
+    *vpt = v;
+    *tpr = (int)(((items + v - 1) / v + 63) / 64 * 64);
+}
+// rows of `part`: two workgroups a CU (one of rows over 512 threads), every one as many rows as the others or one less; up to four rows
+// each before all CUs have two, because a workgroup's share of dw is written and read again: as many bytes as a row and a half
 static inline int rms_bwd_grid(int64_t rows, int tpr) {
-    const int64_t want = tpr == 64 ? (rows + 3) / 4 : rows, most = tpr == 64 ? 512 : tpr <= 320 ? 768 : tpr <= 512 ? 512 : 256;
-    return (int)(want < most ? want : most);
+    const int64_t want = tpr == 64 ? (rows + 3) / 4 : rows, most = tpr <= 512 ? 512 : 256, few = (want + 255) / 256;
+    int64_t each = (want + most - 1) / most;
+    if (each < 4) each = few < 4 ? few : 4;
+    return (int)((want + each - 1) / each);
 }
 extern "C" int64_t edadm_rmsnorm_bwd_ws_floats(int64_t rows, int64_t cols) {
     if (rows < 1 || cols < 1 || cols > RMS_MAX_COLS) return 0;
     int vpt, tpr;
     const int64_t items = mx_blocks(cols) * 4;
-    rms_shape(rows, items, &vpt, &tpr);
+    rms_bwd_shape(rows, items, &vpt, &tpr);
     return (int64_t)rms_bwd_grid(rows, tpr) * (tpr == 64 ? 4 : 1) * items * 8;
 }
 extern "C" int edadm_rmsnorm_bwd(const void* gy, int64_t ldg, const void* gh, int64_t ldgh, const void* h, int64_t ldh, int dt,
@@ -464,20 +473,28 @@ extern "C" int edadm_rmsnorm_bwd(const void* gy, int64_t ldg, const void* gh, in
                      mx_vec(weight, 0, dt, 1) && mx_vec(dh, ldd, dt, rows);
     const int64_t items = mx_blocks(cols) * 4;
     int vpt, tpr;
-    rms_shape(rows, items, &vpt, &tpr);
+    rms_bwd_shape(rows, items, &vpt, &tpr);
     const int per = tpr == 64 ? 4 : 1, grid = rms_bwd_grid(rows, tpr);
     hipStream_t st = (hipStream_t)stream;
     const bool wf32 = weight_f32 || dt == MX_F32;
-#define RMS_GO(W, P, V) k_rmsnorm_bwd<DT, W, P, V><<<grid, tpr * per, 0, st>>>(gy, ldg, gh, ldgh, h, ldh, rstd, weight, dh, ldd, dw ? ws : nullptr, rows, cols, (int)items, fmt, tpr)
+#define RMS_GO(W, P, V)                                                                                                          \
+    do {                                                                                                                         \
+        if constexpr (P == 4) {                                                                                                  \
+            if (tpr > 512) { RMS_ONE(W, P, V, 1024); break; }                                                                    \
+        }                                                                                                                        \
+        RMS_ONE(W, P, V, 512);                                                                                                   \
+    } while (0)
+#define RMS_ONE(W, P, V, T) k_rmsnorm_bwd<DT, W, P, V, T><<<grid, tpr * per, 0, st>>>(gy, ldg, gh, ldgh, h, ldh, rstd, weight, dh, ldd, dw ? ws : nullptr, rows, cols, (int)items, fmt, tpr)
 #define RMS_V(W, V) do { if (vpt == 1) RMS_GO(W, 1, V); else if (vpt == 2) RMS_GO(W, 2, V); else RMS_GO(W, 4, V); } while (0)
     if (rows) MX_DT(dt, {
         if (wf32) { if (vec) RMS_V(true, true); else RMS_V(true, false); }
-        else { if (vec) RMS_V(false, true); else RMS_V(false, false); }
+        else if constexpr (DT != MX_F32) { if (vec) RMS_V(false, true); else RMS_V(false, false); }
     })
 #undef RMS_V
+#undef RMS_ONE
 #undef RMS_GO
     if (dw) {
-        const unsigned g = (unsigned)((cols + 31) / 32);
+        const unsigned g = (unsigned)((cols + 15) / 16);
         const int n = rows ? grid * per : 0;
         if (wf32) k_colsum<MX_F32><<<g, 1024, 0, st>>>(ws, items * 8, n, dw, cols);
         else if (dt == MX_BF16) k_colsum<MX_BF16><<<g, 1024, 0, st>>>(ws, items * 8, n, dw, cols);

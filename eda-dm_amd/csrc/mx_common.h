@@ -159,3 +159,32 @@ template <int FMT> __device__ __forceinline__ void mx_put(uint8_t* codes, uint8_
     else *(uint2*)(codes + item * 8) = c;
     if ((item & 3) == 0) scales[item >> 2] = (uint8_t)b;
 }
+
+// 8 elements as they come from memory, unpacked later: what a kernel holds of a row it has not begun
+template <int DT, bool VEC> struct mx_raw {
+    uint32_t u[VEC ? (DT == MX_F32 ? 8 : 4) : 8];
+};
+template <int DT, bool VEC> __device__ __forceinline__ void mx_fetch8(const void* p, int64_t at, int valid, mx_raw<DT, VEC>& r) {
+    if constexpr (VEC) {
+        const uint4* q = (const uint4*)((const char*)p + at * mx_size<DT>::v);
+#pragma unroll
+        for (int k = 0; k < (DT == MX_F32 ? 2 : 1); ++k) {
+            const uint4 a = q[k];
+            r.u[4 * k] = a.x; r.u[4 * k + 1] = a.y; r.u[4 * k + 2] = a.z; r.u[4 * k + 3] = a.w;
+        }
+    } else {
+        float v[8];
+        mx_load8<DT, false>(p, at, valid, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r.u[e] = __float_as_uint(v[e]);
+    }
+}
+template <int DT, bool VEC> __device__ __forceinline__ void mx_unpack8(const mx_raw<DT, VEC>& r, float (&v)[8]) {
+    if constexpr (VEC && DT != MX_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[2 * e] = mx_lo(r.u[e], DT); v[2 * e + 1] = mx_hi(r.u[e], DT); }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.u[e]);
+    }
+}
