@@ -1144,7 +1144,11 @@ def mx_fake_quant_bwd(gy, x, fmt):
     f, dt = _mx_fmt(fmt), _mx_dt(x)
     if gy.shape != x.shape or gy.dtype != x.dtype:
         raise lib.EdadmError("gradient of %s %s for an input of %s %s" % (gy.dtype, tuple(gy.shape), x.dtype, tuple(x.shape)))
-    dev = _mx_device(x, gy)
+    return _mx_fake_bwd(gy, x, f, dt, _mx_device(x, gy))
+
+
+def _mx_fake_bwd(gy, x, f, dt, dev):
+    """mx_fake_quant_bwd behind its checks (autograd has made them: a gradient has its output's shape, type and device)"""
     r, rows, cols, ld = _mx_rows(x)
     g, _, _, ldg = _mx_rows(gy)
     out = x.new_empty(x.shape)
@@ -1206,19 +1210,22 @@ def rmsnorm_bwd(gy, gh, h, rstd, weight, fmt=None, need_dw=True):
     dt, w, wf32 = _rms_args(h, weight, 0.0, gh)
     if gy.shape != h.shape or gy.dtype != h.dtype:
         raise lib.EdadmError("gradient of %s %s for a stream of %s %s" % (gy.dtype, tuple(gy.shape), h.dtype, tuple(h.shape)))
-    f = 0 if fmt is None else _mx_fmt(fmt)
-    dev = _mx_device(h, gy, gh, rstd, w)
+    if rstd.dtype != torch.float32 or rstd.numel() * h.shape[-1] != h.numel() or not rstd.is_contiguous():
+        raise lib.EdadmError("rstd [%d] in float32 expected" % (h.numel() // h.shape[-1]))
+    return _rmsnorm_bwd(gy, gh, h, rstd, w, wf32, 0 if fmt is None else _mx_fmt(fmt), dt, _mx_device(h, gy, gh, rstd, w), need_dw)
+
+
+def _rmsnorm_bwd(gy, gh, h, rstd, w, wf32, f, dt, dev, need_dw):
+    """rmsnorm_bwd behind its checks (autograd has made them)"""
     r, rows, cols, ldh = _mx_rows(h)
-    if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
-        raise lib.EdadmError("rstd [%d] in float32 expected" % rows)
     g, _, _, ldg = _mx_rows(gy)
     up, _, _, ldgh = _mx_rows(gh) if gh is not None else (None, 0, 0, 0)
     dh = h.new_empty(h.shape)
     if rows == 0:
-        return dh, torch.zeros_like(weight) if need_dw else None
+        return dh, torch.zeros_like(w) if need_dw else None
     dw = ws = None
     if need_dw:
-        dw = h.new_empty(cols, dtype=weight.dtype)
+        dw = h.new_empty(cols, dtype=w.dtype)
         ws = h.new_empty(lib.load().edadm_rmsnorm_bwd_ws_floats(rows, cols), dtype=torch.float32)
     _mx_call(dev, "edadm_rmsnorm_bwd", g.data_ptr(), ldg, None if up is None else up.data_ptr(), ldgh, r.data_ptr(), ldh, dt, rstd.data_ptr(),
              w.data_ptr(), wf32, dh.data_ptr(), cols, dw.data_ptr() if need_dw else None, ws.data_ptr() if need_dw else None, rows, cols, f)

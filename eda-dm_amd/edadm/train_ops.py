@@ -240,14 +240,15 @@ class _MxFakeQuantFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, fmt):
         ctx.save_for_backward(x)
-        ctx.fmt = fmt
-        return ops.mx_fake_quant_fwd(x, fmt)
+        y = ops.mx_fake_quant_fwd(x, fmt)                  # refuses what the backward could not take
+        ctx.meta = ops._MX_FMT[fmt], ops._MX_DT[x.dtype], x.get_device()
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
         (x,) = ctx.saved_tensors
-        return ops.mx_fake_quant_bwd(gy, x, ctx.fmt), None
+        return ops._mx_fake_bwd(gy, x, *ctx.meta), None
 
 
 def mx_fake_quant(x, fmt):
@@ -262,7 +263,8 @@ class _RmsNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, eps, fmt, residual):
         y, h, rstd = ops.rmsnorm_fwd(x, weight, eps, fmt, residual, fake=fmt is not None, want_rstd=True)
         ctx.save_for_backward(h, weight, rstd)
-        ctx.fmt, ctx.two = fmt, residual is not None
+        ctx.meta = (1 if weight.dtype == torch.float32 else 0, 0 if fmt is None else ops._MX_FMT[fmt], ops._MX_DT[x.dtype], x.get_device())
+        ctx.two = residual is not None
         ctx.set_materialize_grads(False)
         return (y, h) if ctx.two else y
 
@@ -274,7 +276,7 @@ class _RmsNormFn(torch.autograd.Function):
         if gy is None:                                     # only the stream went on: its gradient passes through the addition
             return (gh if need[0] else None, torch.zeros_like(weight) if need[1] else None, None, None,
                     gh if ctx.two and need[4] else None)
-        dh, dw = ops.rmsnorm_bwd(gy, gh, h, rstd, weight, ctx.fmt, need_dw=need[1])
+        dh, dw = ops._rmsnorm_bwd(gy, gh, h, rstd, weight.contiguous(), *ctx.meta, need[1])
         return dh if need[0] else None, dw, None, None, dh if ctx.two and need[4] else None
 
 
