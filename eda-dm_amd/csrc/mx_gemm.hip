@@ -1,10 +1,14 @@
-// Product of microscaled operands on the block-scaled matrix instructions (v_mfma_scale_f32_16x16x128_f8f6f4):
+// Product of microscaled operands on the block-scaled matrix instructions (v_mfma_scale_f32_16x16x128_f8f6f4, .._32x32x64_..):
 //   out[m][n] = sum_b 2^(sa[m][b] - 127 + sw[n][b] - 127) sum_{k in block b} a[m][k] w[n][k]  (+ bias[n])
 // with a in e4m3 or e2m1 and w in e2m1, both as they lie in memory (rows of blocks; no weight is re-packed), 32-bit accumulation.
 //
-// Operand layout of the 16 x 16 x 128 instruction, lane l = 16 q + r: a 4-bit operand's lane holds the 32 elements of block q of
-// row r; an 8-bit operand's lane holds elements 16 q .. 16 q + 15 of each half of row r; either way lane l gives the scale of
-// block q of row r.  w goes in as the first operand, so that a lane ends up with four neighbouring columns of one output row.
+// Operand layout of the 16 x 16 x 128 (32 x 32 x 64) instruction, lane l = 16 q + r (32 q + r): a 4-bit operand's lane holds the 32
+// elements of block q of row r; an 8-bit operand's lane holds elements 16 q .. 16 q + 15 of each half of row r; either way lane l gives
+// the scale of block q of row r.  w goes in as the first operand, so that a lane ends up with four neighbouring columns of one output row.
+//
+// What bounds it: one to 32 rows, reading w (k_mx_rows); few tiles, the way to memory (k_mx_stream); many, the matrix cores and the
+// clock they leave (k_mx_tile): the instructions alone, operands in registers, reach 3.6 PFLOP/s with 8-bit a (1.72 GHz held) and 6.6
+// with 4-bit a (1.58 GHz); 8192 x 10240 x 5120 runs at 2.5 (8-bit), 8192 x 8192 x 8192 at 3.9 (4-bit).
 //
 // Precision.  Within a group of products the instruction keeps 13 binary places below the largest exponent.  The 4 x 4-bit products
 // (and 8 x 4-bit ones within 8 binades) are inside that and sum exactly; e4m3 spans 18 binades, and what falls below is cut off: a
@@ -100,7 +104,9 @@ template <int ODT> __device__ __forceinline__ void mx_out4(const MxArgs& a, int6
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup owns 16 MT rows and 16 NT columns; its waves (as many as the launch gives it) take pairs of K-steps of 128 in turn, so
 // that every cache line of w (128 bytes = a pair of a row) is read by one wave, fetch their operands straight into registers, a pair
-// ahead of the one they multiply, and add their sums in LDS in the order of the waves.  Bound by reading w once.
+// ahead of the one they multiply, and add their sums in LDS in the order of the waves.  Bound by reading w once: 1 x 5120 x 5120 6.9 us
+// in a graph (3.4 of them what any launch takes; 13.9 MB), 1 x 10240 x 10240 16.4 us, 4.3 TB/s behind the launch.  Every load is made
+// without a condition (a conditional 16-byte load was split into four).
 typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
 typedef uint32_t mx_u64 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
@@ -247,9 +253,13 @@ __global__ __launch_bounds__(64 * MAXW) void k_mx_rows(MxArgs a, int strips) {
 //
 // Hand-off: one barrier a step, in front of its last sub-step.  Behind it the next step's operands are complete for every wave, so that
 // their first fragments are fetched while the last sub-step multiplies, and the load of the step after next goes out, a full step
-// ahead of its use.  8-bit a: three slots of 48 KB; that load fills the slot of the step before, which no wave reads any more, and a
-// fragment of a is fetched over the one just used (two sets of them and the sums would not fit 256 registers).  4-bit a: two slots of
-// 64 KB; the load fills this step's slot, so its last fragments are awaited in front of the barrier, and there are two sets.
+// ahead of its use.  8-bit a: three slots (48 KB at 256 x 256); that load fills the slot of the step before, which no wave reads any
+// more.  4-bit a: two slots (64 KB); it fills this step's slot, so the step's last fragments are awaited in front of the barrier, and
+// half of it goes out in the next sub-step, whose multiplications are half as long as the loads' issue.  One wave a SIMD with a quarter of
+// the tile (128 x 128 at most: 256 sums, two sets of fragments): eight waves of half as much read a half more from LDS and spilled.
+//
+// Everything that is fetched is fetched behind a multiplication (`step`), pinned there: a branch or a free order cost a third of the
+// rate (712 -> 470 us at 8192 x 10240 x 5120, 8-bit a), a load of scales a step another quarter (-> 340).
 //
 // LDS order: 16-byte piece p of row r lies at piece p ^ ((r >> 1) & 7) (rows of 128 bytes) or p ^ ((r >> 2) & 3) (rows of 64), so that
 // the 16 lanes of a quarter of a fragment read hit 16 different 16-byte groups of banks; the loads permute their source addresses.
@@ -400,7 +410,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     constexpr int ABYTES = BM * 128, WBYTES = BN * WROW, STAGE = ABYTES + WBYTES;
     constexpr int RING = AF == MX_FP4 ? 2 : 3;                        // steps' operands in LDS
     constexpr int AI = ABYTES / (THREADS * 16), WI = WBYTES / (THREADS * 16);   // load instructions a wave
-    constexpr int LOADS = AI + WI, EARLY = AF == MX_FP4 ? LOADS / 2 : LOADS;                  // those sent out behind the barrier of the step before
+    constexpr int LOADS = AI + WI, EARLY = AF == MX_FP4 ? LOADS / 2 : LOADS;    // those sent out behind the barrier of the step before
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
         for (int d = 0; d < SD; ++d) grp[e][d] = *(const mx_u32*)(row_at(e, step) + 4 * d);
     };
-    // the next step's scales from place k of a group, then (NEW) the next group in the old one's place
+    // the next step's scales from place k of a group; at its end from the next group, which then takes its place
     auto shift1 = [&](int e, int k, bool turn_over) {
 #pragma unroll
         for (int d = 0; d < SD; ++d) nx[e][d] = (turn_over ? far[e][d] : grp[e][k * SD + d]) >> (8 * q);
@@ -530,8 +540,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
         int at = 0, next = STAGE, fill = RING == 3 ? 2 * STAGE : 0;
         // one step; MORE steps behind it (0, 1 or at least 2) decide what is fetched; PLACE: the step's place in its group, -1 for a step
-        // behind the last whole group.  No branch inside: the compiler would move a
-        // sub-step's multiplications behind it, away from the fetches they hide
+        // behind the last whole group.  No branch inside: the compiler would move a sub-step's multiplications behind it, away from the
+        // fetches they hide
         auto step = [&](int s, auto more, auto place) {
             constexpr int MORE = decltype(more)::value, PLACE = decltype(place)::value;
             mx_unroll<SUB>([&](auto tt) {

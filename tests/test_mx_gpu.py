@@ -453,6 +453,21 @@ def test_product_reads_and_writes_only_its_own(ops, fmt, m):
     assert bool((out == 7.0).all())
 
 
+def test_product_past_two_gigabytes(ops):
+    """rows of a and of the output whose offsets pass 2^31 bytes and elements: the first and the last ones against the reference"""
+    m, n, k = 280_000, 8200, 8192
+    a = ops.mx_quantize(torch.zeros(m, k, dtype=torch.bfloat16, device="cuda"), "mxfp8")
+    some = ops.mx_quantize(data((40, k), torch.float32, 6).cuda(), "mxfp8")
+    w = ops.mx_quantize(data((n, k), torch.float32, 7, 0.2).cuda() * 0.02, "mxfp4")
+    assert a.codes.numel() > 2 ** 31 and m * n > 2 ** 31
+    a.codes[:20], a.codes[-20:] = some.codes[:20], some.codes[20:]
+    a.scales[:20], a.scales[-20:] = some.scales[:20], some.scales[20:]
+    va, vw = ops.mx_dequantize(some).double(), ops.mx_dequantize(w).double()
+    out = ops.mx_gemm(a, w)
+    check_product(torch.cat([out[:20], out[-20:]]), va, vw, None, torch.bfloat16, "mxfp8")
+    assert int(torch.count_nonzero(out[20:-20:997])) == 0
+
+
 # ------------------------------------------------------------------------------------------------ together
 def block_chain(ops, x, res, nw, w1, w2, fmt):
     q, h = ops.rmsnorm_mx(x, nw, 1e-6, fmt, residual=res)
