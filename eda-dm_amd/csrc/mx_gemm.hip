@@ -279,9 +279,9 @@ __device__ __forceinline__ void mx_dma4(const void* base, uint32_t voff, uint32_
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
 
-// everything in flight from memory has arrived (LDS: and from LDS); a form the compiler knows, so that it does not wait again for loads
-// that it would find behind newer ones
-template <bool LDS> __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(LDS ? 0x0070 : 0x0f70); }
+// all but the newest N loads from memory, and all from LDS, have arrived; a form the compiler knows, so that after N = 0 it does not wait
+// again for loads that it would find behind newer ones
+template <int N> __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14); }
 
 // index of this workgroup's tile: workgroups go round the 8 XCDs, so every XCD gets a run of neighbouring tiles, which share operands in
 // its L2
@@ -410,7 +410,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     constexpr int ABYTES = BM * 128, WBYTES = BN * WROW, STAGE = ABYTES + WBYTES;
     constexpr int RING = AF == MX_FP4 ? 2 : 3;                        // steps' operands in LDS
     constexpr int AI = ABYTES / (THREADS * 16), WI = WBYTES / (THREADS * 16);   // load instructions a wave
-    constexpr int LOADS = AI + WI, EARLY = AF == MX_FP4 ? LOADS / 2 : LOADS;    // those sent out behind the barrier of the step before
+    constexpr int LOADS = AI + WI, EARLY = LOADS / 2;              // those sent out in a step's last sub-step
+    constexpr int LAG = RING - 2;                                     // steps a load has besides the one it is due in
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
             if (grouped) far1(e, 0);
             else one1(e, 0);
         }
-        mx_wait<RING == 2>();
+        mx_wait<0>();
         __builtin_amdgcn_s_barrier();
 #pragma unroll
         for (int e = 0; e < ROWS; ++e) shift1(e, 0, grouped);
@@ -529,17 +530,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
             for (int e = 0; e < ROWS; ++e) one1(e, 1);
         }
-        if (steps > 1) {
+        if (LAG && steps > 1) load(STAGE);
+        if (steps > 1 + LAG) {
 #pragma unroll
-            for (int l = 0; l < EARLY; ++l) load1(STAGE, l);
-            if (EARLY == LOADS) advance();
+            for (int l = 0; l < EARLY; ++l) load1((1 + LAG) * STAGE, l);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) fx[0][i] = fragx(0, 0, i);
 #pragma unroll
         for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
-        int at = 0, next = STAGE, fill = RING == 3 ? 2 * STAGE : 0;
-        // one step; MORE steps behind it (0, 1 or at least 2) decide what is fetched; PLACE: the step's place in its group, -1 for a step
+        int at = 0, next = STAGE, last = LAG ? 2 * STAGE : STAGE;     // slots of this step, the next and the newest that is being loaded
+        // one step; MORE steps behind it (0 .. 2 or at least 3) decide what is fetched; PLACE: the step's place in its group, -1 for a step
         // behind the last whole group.  No branch inside: the compiler would move a sub-step's multiplications behind it, away from the
         // fetches they hide
         auto step = [&](int s, auto more, auto place) {
@@ -548,17 +549,20 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                 constexpr int t = decltype(tt)::value, nt = (t + 1) % SUB, fb = t & 1;
                 constexpr bool LAST = t == SUB - 1;
                 if constexpr (LAST && MORE > 0) {
+                    // newer than the next step's operands: those of the step after (three slots) and a group's scales; at the end of a
+                    // group its scales are due too, and behind the last group nobody counts
+                    constexpr int NEWER = LAG == 0 || PLACE < 0 || PLACE == GS - 1 ? 0 : LOADS + (PLACE == 1 ? ROWS : 0);
                     asm volatile("" ::: "memory");
-                    mx_wait<RING == 2>();
+                    mx_wait<NEWER>();
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                 }
-                // behind each multiplication: a fragment for the next sub-step; a load instruction, of the step after next behind the
-                // barrier, what is left of the next step's in the first sub-step; a row of the next step's scales (awaited at the
-                // barrier) and the load of a row of scales
+                // behind each multiplication: a fragment for the next sub-step; a load instruction, the first half of a step's behind the
+                // barrier, the second in the next step's first sub-step; a row of the next step's scales (awaited at the barrier) and the
+                // load of a row of scales
                 const int from = LAST ? next : at;
                 constexpr int OPS = MT * NT, READS = !LAST || MORE > 0 ? MT + NT : 0, SHIFTS = LAST && MORE > 0 ? ROWS : 0;
-                constexpr int LOW = LAST ? 0 : EARLY, FILL = LAST && MORE > 1 ? EARLY : t == 0 && MORE > 0 ? LOADS - EARLY : 0;
+                constexpr int LOW = LAST ? 0 : EARLY, FILL = LAST && MORE > 1 + LAG ? EARLY : t == 0 && MORE > LAG ? LOADS - EARLY : 0;
                 mx_unroll<OPS>([&](auto kk) {
                     constexpr int k = decltype(kk)::value, i = k / NT, j = k % NT;
                     acc[i][j] = mx_mma32<AF, EXACT, t>(fw[fb][j], fx[fb][i], acc[i][j], sc[MT + j][t / 2], sc[i][t / 2]);
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                         if constexpr (e < NT) fw[fb ^ 1][e] = fragw(from, nt, e);
                         else fx[fb ^ 1][e - NT] = fragx(from, nt, e - NT);
                     });
-                    mx_unroll<(k + 1) * FILL / OPS - k * FILL / OPS>([&](auto dd) { load1(LAST ? fill : next, LOW + k * FILL / OPS + decltype(dd)::value); });
+                    mx_unroll<(k + 1) * FILL / OPS - k * FILL / OPS>([&](auto dd) { load1(LAST ? at : last, LOW + k * FILL / OPS + decltype(dd)::value); });
                     mx_unroll<(k + 1) * SHIFTS / OPS - k * SHIFTS / OPS>([&](auto dd) {
                         constexpr int e = k * SHIFTS / OPS + decltype(dd)::value;
                         shift1(e, PLACE < 0 ? 0 : PLACE + 1, PLACE == GS - 1);
@@ -576,16 +580,16 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                     });
                     __builtin_amdgcn_sched_barrier(0);
                 });
-                if constexpr (FILL && (LAST ? EARLY == LOADS : true)) advance();
+                if constexpr (FILL && !LAST) advance();
             });
             if constexpr (MORE > 0) take();
             const int keep = at;
             at = next;
-            if constexpr (RING == 2) { next = keep; fill = at; }
-            else { next = fill; fill = keep; }
+            next = LAG ? last : keep;
+            last = keep;
         };
         int s = 0;
-        for (; s + 2 * GS <= steps; s += GS) mx_unroll<GS>([&](auto place) { step(s + decltype(place)::value, mx_int<2>{}, place); });
+        for (; s + 2 * GS <= steps; s += GS) mx_unroll<GS>([&](auto place) { step(s + decltype(place)::value, mx_int<3>{}, place); });
         if (grouped) {                                                // the step behind next is in the group at hand
 #pragma unroll
             for (int d = 0; d < SD; ++d) {
@@ -593,7 +597,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                 for (int e = 0; e < ROWS; ++e) grp[e][d] = grp[e][SD + d];
             }
         }
-        for (; s + 2 < steps; ++s) step(s, mx_int<2>{}, mx_int<-1>{});
+        for (; s + 3 < steps; ++s) step(s, mx_int<3>{}, mx_int<-1>{});
+        if (s + 2 < steps) step(s++, mx_int<2>{}, mx_int<-1>{});
         if (s + 1 < steps) step(s++, mx_int<1>{}, mx_int<-1>{});
         step(s, mx_int<0>{}, mx_int<-1>{});
     }
