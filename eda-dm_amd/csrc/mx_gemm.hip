@@ -753,18 +753,25 @@ template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static in
 template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hipStream_t st) {
     // the tiled kernel's 32-bit row offsets: 256 rows of a and of w under 4 GB
     const bool fits = a.lda < (1 << 23) && a.ldw < (1 << 23) && a.ldas < (1 << 23) && a.ldws < (1 << 23);
+    // few rows: 32 x 5120 x 5120 10.6 us there and 12.2 on 64 x 64 tiles, 48 x 5120 x 5120 13.6 and 12.4
     if (a.M <= 32 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
-    // The tile is the one of least cost: tiles a CU x what a tile costs on a full chip, and no less than what one costs alone (both
-    // in units of a 256 x 256 tile on a full chip, 68 us at K = 5120 with 8-bit a, 44 us with 4-bit a; measured over M = 64 .. 8192,
-    // the ratios are the same for both).  4096 x 5120 x 5120: 256 x 256 leaves three quarters of the second round empty (81 us, 4-bit
-    // a), 256 x 192 takes 69;  8192 x 10240 x 5120: 339 against 369 us, 8-bit a;  256 x 5120 x 5120: 64 x 64 takes 15.6 us, 256 x 256 49.
-    static const struct { int bm, bn; float full, alone; } tiles[] = {
-        {256, 256, 1.f, 0.75f}, {256, 192, 0.805f, 0.65f}, {128, 128, 0.33f, 0.40f}, {64, 128, 0.19f, 0.22f}, {64, 64, 0.116f, 0.19f}};
+    // The tile of least cost, in microseconds with 8-bit a and k = K / 1024 (4-bit a: two thirds of k): t tiles a CU of a full chip take
+    // t (a + b k), and few tiles are no faster than c + d k min(t, r), r of them sharing a CU while they wait for memory.  Constants fitted
+    // to 40 shapes (M 64 .. 32768, N 320 .. 10240, K 64 .. 10240), two sides of each choice: 8192 x 10240 x 5120 339 us on 256 x 256 and 369
+    // on 256 x 192; 4096 x 5120 x 5120, 4-bit a, 81 and 69; 8192 x 8192 x 512 75 on 256 x 256, whose start and way out nothing hides, and 59
+    // on 128 x 128, two of which share a CU; 600 x 3000 x 8000 48 on 128 x 128 and 38 on 64 x 128; 128 x 5120 x 5120 15 on 64 x 128, 13 on
+    // 64 x 64.
+    static const struct { int bm, bn; float a, b, c, d; int r; } tiles[] = {{256, 256, 13.f, 11.f, 10.f, 8.5f, 1},
+                                                                          {256, 192, 9.f, 8.7f, 8.f, 7.f, 1},
+                                                                          {128, 128, 1.5f, 4.25f, 3.f, 4.9f, 1},
+                                                                          {64, 128, 1.05f, 2.3f, 3.f, 2.8f, 2},
+                                                                          {64, 64, 0.5f, 1.5f, 3.f, 1.9f, 3}};
+    const float k = (float)a.nblk * (AF == MX_FP4 ? 0.66f / 32 : 1.f / 32);
     int pick = 0;
     float best = 0;
     for (int i = 0; i < 5; ++i) {
-        const int64_t n = ((a.M + tiles[i].bm - 1) / tiles[i].bm) * ((a.N + tiles[i].bn - 1) / tiles[i].bn);
-        const float cost = fmaxf(tiles[i].alone, tiles[i].full * (float)((n + 255) / 256));
+        const int64_t n = ((a.M + tiles[i].bm - 1) / tiles[i].bm) * ((a.N + tiles[i].bn - 1) / tiles[i].bn), t = (n + 255) / 256;
+        const float few = tiles[i].c + tiles[i].d * k * (float)(t < tiles[i].r ? t : tiles[i].r), cost = fmaxf(few, (float)t * (tiles[i].a + tiles[i].b * k));
         if (i == 0 || cost < best) { best = cost; pick = i; }
     }
     switch (pick) {

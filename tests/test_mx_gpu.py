@@ -383,6 +383,22 @@ def test_product_tiles(ops, mn, k, fmt):
         assert torch.equal(ops.mx_gemm(a, w, bias=bias, dtype=dtype), got)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("k", [1280, 1408, 1664, 2016, 2592, 2816, 3040, 3330, 3616, 4224])
+@pytest.mark.parametrize("mn", [(4096, 4096), (4000, 4090), (2048, 5120), (1900, 5001)])
+def test_product_long_rows(ops, mn, k, fmt):
+    """the 256-row tiles over K with every remainder of whole steps (four or two to a group of scales) and of blocks behind them"""
+    m, n = mn
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    a = ops.mx_quantize(torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(k, generator=g, device="cuda")), fmt)
+    w = ops.mx_quantize(torch.randn(n, k, generator=g, device="cuda") * 0.02, "mxfp4")
+    va, vw = ops.mx_dequantize(a).double(), ops.mx_dequantize(w).double()
+    for dtype in (torch.float32, torch.float16):
+        got = ops.mx_gemm(a, w, dtype=dtype)
+        check_product(got, va, vw, None, dtype, fmt)
+        assert torch.equal(ops.mx_gemm(a, w, dtype=dtype), got)
+
+
 @pytest.mark.parametrize("m", [1, 2, 3, 16, 17, 32, 33])
 @pytest.mark.parametrize("n", [64, 4100, 8200])
 @pytest.mark.parametrize("fmt", FMTS)
