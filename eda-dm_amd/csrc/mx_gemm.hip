@@ -6,8 +6,8 @@
 // elements of block q of row r; an 8-bit operand's lane holds elements 16 q .. 16 q + 15 of each half of row r; either way lane l gives
 // the scale of block q of row r.  w goes in as the first operand, so that a lane ends up with four neighbouring columns of one output row.
 //
-// What bounds it: one to 32 rows, reading w (k_mx_rows); few tiles, the way to memory (k_mx_stream); many, the matrix cores and the
-// clock they leave (k_mx_tile): the instructions alone, operands in registers, reach 3.6 PFLOP/s with 8-bit a (1.72 GHz held) and 6.6
+// What bounds it: one to 32 rows, reading w (k_mx_rows); few tiles, the way to memory; many, the matrix cores and the clock they leave
+// (k_mx_tile): the instructions alone, operands in registers, reach 3.6 PFLOP/s with 8-bit a (1.72 GHz held) and 6.6
 // with 4-bit a (1.58 GHz); 8192 x 10240 x 5120 runs at 2.5 (8-bit), 8192 x 8192 x 8192 at 4.0 (4-bit).
 //
 // Precision.  Within a group of products the instruction keeps 13 binary places below the largest exponent.  The 4 x 4-bit products
@@ -275,11 +275,6 @@ __device__ __forceinline__ void mx_dma16(const void* base, uint32_t voff, uint32
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
 
-// the same, 4 bytes a lane
-__device__ __forceinline__ void mx_dma4(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
-}
-
 // all but the newest N loads from memory, and all from LDS, have arrived; a form the compiler knows, so that after N = 0 it does not wait
 // again for loads that it would find behind newer ones
 template <int N> __device__ __forceinline__ void mx_wait() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14); }
@@ -478,7 +473,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     for (int j = 0; j < NT; ++j) wso[j] = (uint32_t)min((int64_t)((wn * NT + j) * 32 + r), a.N - 1 - n0) * (uint32_t)a.ldws;
     // A load of scales touches a cache line a row, so it costs the same for one step's bytes as for 16: those of GS steps are loaded
     // together (a load a step took a quarter of the kernel's time).  Rows e < MT are a's, the others w's.  grp: the current group's, as
-    // loaded;  far: the next group's;  sc: this step's, shifted to the lane's half;  nx: the next step's
+    // loaded;  far: the next group's;  sc: this step's, shifted to the lane's half;  nx: the next step's.  The last GS to 2 GS - 1 steps
+    // take theirs from the front of grp, which moves up, and so load none; what does not make a group behind the last whole one comes from
+    // the row's last group of bytes (4096 x 5120 x 5120, 8-bit a: 101 -> 97 us against a load a step there, 128 x 5120 x 5120 11.3 -> 10.5)
     constexpr int SD = STEP / 4;                                      // dwords of scales a row and step
     constexpr int GS = 4 / SD, ROWS = MT + NT;                        // steps a group
     uint32_t grp[ROWS][4], far[ROWS][4], nx[ROWS][SD], sc[ROWS][SD];
@@ -488,10 +485,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
         for (int d = 0; d < 4; ++d) far[e][d] = u[d];
     };
-    // one step's bytes, into the group's first place: the steps behind the last whole group
-    auto one1 = [&](int e, int step) {
+    auto up1 = [&](int e) {
 #pragma unroll
-        for (int d = 0; d < SD; ++d) grp[e][d] = *(const mx_u32*)(row_at(e, step) + 4 * d);
+        for (int d = 0; d + SD < 4; ++d) grp[e][d] = grp[e][d + SD];
     };
     // the next step's scales from place k of a group; at its end from the next group, which then takes its place
     auto shift1 = [&](int e, int k, bool turn_over) {
@@ -530,21 +526,19 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     if (steps) {
         mx_i8 fx[2][MT], fw[2][NT];
         load(0);
-        const bool grouped = steps >= 2 * GS;
 #pragma unroll
         for (int e = 0; e < ROWS; ++e) {
-            if (grouped) far1(e, 0);
-            else one1(e, 0);
+            if (steps >= GS) far1(e, 0);
+            else {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) far[e][d] = *(const mx_u32*)(row_at(e, 0) + 4 * min(d, steps * SD - 1));
+            }
         }
         mx_wait<0>();
         __builtin_amdgcn_s_barrier();
 #pragma unroll
-        for (int e = 0; e < ROWS; ++e) shift1(e, 0, grouped);
+        for (int e = 0; e < ROWS; ++e) shift1(e, 0, true);
         take();
-        if (!grouped && steps > 1) {
-#pragma unroll
-            for (int e = 0; e < ROWS; ++e) one1(e, 1);
-        }
         if (LAG && steps > 1) load(STAGE);
         if (steps > 1 + LAG) {
 #pragma unroll
@@ -555,8 +549,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
 #pragma unroll
         for (int j = 0; j < NT; ++j) fw[0][j] = fragw(0, 0, j);
         int at = 0, next = STAGE, last = LAG ? 2 * STAGE : STAGE;     // slots of this step, the next and the newest that is being loaded
-        // one step; MORE steps behind it (0 .. 2 or at least 3) decide what is fetched; PLACE: the step's place in its group, -1 for a step
-        // behind the last whole group.  No branch inside: the compiler would move a sub-step's multiplications behind it, away from the
+        // one step; MORE steps behind it (0 .. 2 or at least 3) decide what is fetched; PLACE: the step's place in its group, -1 for one of
+        // the last steps.  No branch inside: the compiler would move a sub-step's multiplications behind it, away from the
         // fetches they hide
         auto step = [&](int s, auto more, auto place) {
             constexpr int MORE = decltype(more)::value, PLACE = decltype(place)::value;
@@ -565,8 +559,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                 constexpr bool LAST = t == SUB - 1;
                 if constexpr (LAST && MORE > 0) {
                     // newer than the next step's operands: those of the step after (three slots) and a group's scales; at the end of a
-                    // group its scales are due too, and behind the last group nobody counts
-                    constexpr int NEWER = LAG == 0 || PLACE < 0 || PLACE == GS - 1 ? 0 : LOADS + (PLACE == 1 ? ROWS : 0);
+                    // group its scales are due too
+                    constexpr int NEWER = LAG == 0 || MORE == 1 || PLACE == GS - 1 ? 0 : LOADS + (PLACE == 1 ? ROWS : 0);
                     asm volatile("" ::: "memory");
                     mx_wait<NEWER>();
                     __builtin_amdgcn_s_barrier();
@@ -591,7 +585,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
                         constexpr int e = k * SHIFTS / OPS + decltype(dd)::value;
                         shift1(e, PLACE < 0 ? 0 : PLACE + 1, PLACE == GS - 1);
                         if constexpr (PLACE == 0) far1(e, s + GS);
-                        if constexpr (PLACE < 0 && MORE > 1) one1(e, s + 2);
+                        if constexpr (PLACE < 0) up1(e);
                     });
                     __builtin_amdgcn_sched_barrier(0);
                 });
@@ -605,15 +599,34 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
         };
         int s = 0;
         for (; s + 2 * GS <= steps; s += GS) mx_unroll<GS>([&](auto place) { step(s + decltype(place)::value, mx_int<3>{}, place); });
-        if (grouped) {                                                // the step behind next is in the group at hand
+        const int odd = steps < GS ? 0 : steps % GS, full = s + GS - 2;   // steps behind the last whole group;  behind `full` grp is empty
+        if (odd) {
 #pragma unroll
-            for (int d = 0; d < SD; ++d) {
-#pragma unroll
-                for (int e = 0; e < ROWS; ++e) grp[e][d] = grp[e][SD + d];
-            }
+            for (int e = 0; e < ROWS; ++e) far1(e, steps - GS);
         }
-        for (; s + 3 < steps; ++s) step(s, mx_int<3>{}, mx_int<-1>{});
-        if (s + 2 < steps) step(s++, mx_int<2>{}, mx_int<-1>{});
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) up1(e);
+        auto refill = [&](int s) {
+            if (!odd || s != full) return;
+            mx_wait<0>();
+#pragma unroll
+            for (int e = 0; e < ROWS; ++e) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) grp[e][d] = far[e][d];
+            }
+            for (int k = odd; k < GS; ++k) {
+#pragma unroll
+                for (int e = 0; e < ROWS; ++e) up1(e);
+            }
+        };
+        for (; s + 3 < steps; ++s) {
+            step(s, mx_int<3>{}, mx_int<-1>{});
+            refill(s);
+        }
+        if (s + 2 < steps) {
+            step(s, mx_int<2>{}, mx_int<-1>{});
+            refill(s++);
+        }
         if (s + 1 < steps) step(s++, mx_int<1>{}, mx_int<-1>{});
         step(s, mx_int<0>{}, mx_int<-1>{});
     }
@@ -621,89 +634,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_tile(MxArgs a, int tm, int 
     static_assert(WM * WN * MxOut<NT, ODT>::BYTES <= RING * STAGE, "");
     __syncthreads();                                                  // every wave is done with the ring
     mx_out_tile<MT, NT, ODT>(a, m0 + wm * MT * 32, n0 + wn * NT * 32, acc, smem + wave * MxOut<NT, ODT>::BYTES);
-}
-
-// ------------------------------------------------------------------------------------------------ a few dozen rows, or few tiles
-// At most a tile a CU and 8-bit a, where one step ahead does not hide the way to memory: 64 x 64 tiles, four waves of one 32 x 32
-// instruction each, steps of 128 elements through a ring of RING slots (an even number), RING - 2 of them in flight.  The scales lie in
-// the ring too (a dword a row and step), so that every wave issues the same PER loads a step and waits for the oldest steps by their count
-// alone; behind the last step that one is loaded again, to keep the count.  Needs scale rows on dword boundaries.
-#define MX_STREAM_RING 6
-#define MX_STREAM_LDS (MX_STREAM_RING * (64 * 128 + 64 * 64 + 512))
-template <bool EXACT, int ODT>
-__global__ __launch_bounds__(256) void k_mx_stream(MxArgs a, int tm) {
-    constexpr int AF = MX_FP8, AROW = 128, ABYTES = 64 * AROW, WBYTES = 64 * 64, STAGE = ABYTES + WBYTES + 512;
-    constexpr int RING = MX_STREAM_RING, AI = ABYTES / 4096, PER = AI + 2;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-    const int lane = threadIdx.x & 63, r = lane & 31, q = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wm = wave >> 1, wn = wave & 1;
-    const int tile = mx_xcd_run(gridDim.x);
-    const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(tile % tm) * 64, n0 = (int64_t)__builtin_amdgcn_readfirstlane(tile / tm) * 64;
-    uint32_t av[AI], wv, sv;
-#pragma unroll
-    for (int i = 0; i < AI; ++i) {
-        const int row = (i * 256 + (int)threadIdx.x) / 8, p = (lane & 7) ^ ((row >> 1) & 7);
-        av[i] = (uint32_t)min((int64_t)row, a.M - 1 - m0) * (uint32_t)a.lda + p * 16;       // past the last row: read that one
-    }
-    {
-        const int row = (int)threadIdx.x / 4, p = (lane & 3) ^ ((row >> 2) & 3);
-        wv = (uint32_t)min((int64_t)row, a.N - 1 - n0) * (uint32_t)a.ldw + p * 16;
-        sv = wn ? (uint32_t)min((int64_t)lane, a.N - 1 - n0) * (uint32_t)a.ldws : (uint32_t)min((int64_t)lane, a.M - 1 - m0) * (uint32_t)a.ldas;
-    }
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    const uint8_t *ab = a.A + m0 * a.lda, *wb = a.W + n0 * a.ldw, *sb = wn ? a.Ws + n0 * a.ldws : a.As + m0 * a.ldas;
-    auto load = [&](int step, int slot) {
-        const uint32_t la = lds0 + slot * STAGE;
-#pragma unroll
-        for (int i = 0; i < AI; ++i) mx_dma16(mx_uniform(ab + (int64_t)step * AROW), av[i], __builtin_amdgcn_readfirstlane(la + i * 4096 + wave * 1024));
-        mx_dma16(mx_uniform(wb + (int64_t)step * 64), wv, __builtin_amdgcn_readfirstlane(la + ABYTES + wave * 1024));
-        mx_dma4(mx_uniform(sb + (int64_t)step * 4), sv, __builtin_amdgcn_readfirstlane(la + ABYTES + WBYTES + wn * 256));   // both wm alike
-    };
-    mx_f16v acc[1][1];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
-    // two steps at a time: the barrier, the way to LDS and back and the refill cost as much as the multiplications of both
-    const int steps = a.nblk / 4 & ~1;
-    if (steps) {
-        const int sx = (r >> 1) & 7, sz = (r >> 2) & 3;
-        const uint8_t *pa = smem + (wm * 32 + r) * AROW, *pw = smem + ABYTES + (wn * 32 + r) * 64, *ps = smem + ABYTES + WBYTES + r * 4;
-#pragma unroll
-        for (int d = 0; d < RING - 2; ++d) load(min(d, steps - 1), d);
-        int slot = 0, fill = RING - 2;
-        for (int s = 0; s < steps; s += 2) {
-            // (this wave's reads of the slots refilled below arrived before they were multiplied: the count says so to whoever moves code)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER * (RING - 4)) : "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            mx_i8 fx[2][2], fw[2][2];
-            uint32_t sa[2], sw[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = (slot + h) * STAGE;
-                sa[h] = *(const uint32_t*)(ps + at + wm * 128) >> (8 * q);
-                sw[h] = *(const uint32_t*)(ps + at + 256 + wn * 128) >> (8 * q);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    fw[h][t] = frag4(*(const mx_i4*)(pw + at + ((2 * t + q) ^ sz) * 16));
-                    fx[h][t] = frag8(*(const mx_i4*)(pa + at + ((4 * t + q) ^ sx) * 16), *(const mx_i4*)(pa + at + ((4 * t + 2 + q) ^ sx) * 16));
-                }
-            }
-            // the slots of the two steps before: every wave has multiplied what it read there
-            load(min(s + RING - 2, steps - 1), fill);
-            load(min(s + RING - 1, steps - 1), fill + 1);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                acc[0][0] = mx_mma32<AF, EXACT, 0>(fw[h][0], fx[h][0], acc[0][0], sw[h], sa[h]);
-                acc[0][0] = mx_mma32<AF, EXACT, 1>(fw[h][1], fx[h][1], acc[0][0], sw[h], sa[h]);
-            }
-            slot = slot + 2 == RING ? 0 : slot + 2;
-            fill = fill + 2 == RING ? 0 : fill + 2;
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // the loads that kept the count
-    }
-    mx_rest<AF, 1, 1, EXACT>(a, steps * 4, m0 + wm * 32, n0 + wn * 32, acc);
-    __syncthreads();
-    mx_out_tile<1, 1, ODT>(a, m0 + wm * 32, n0 + wn * 32, acc, smem + wave * MxOut<1, ODT>::BYTES);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -779,21 +709,8 @@ template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hip
         case 1: return launch_tile<AF, 2, 2, 4, 3, EXACT, ODT>(a, st);
         case 2: return launch_tile<AF, 2, 2, 2, 2, EXACT, ODT>(a, st);
         case 3: return launch_tile<AF, 2, 2, 1, 2, EXACT, ODT>(a, st);
-        default: break;
+        default: return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
     }
-    // 8-bit a, at most one 64 x 64 tile a CU: the deep ring (48 x 10240 x 5120 12.8 against 15.6 us, 64 x 10240 x 10240 31 against 41);
-    // more of them: four of the plain ring's workgroups fit a CU and hide each other's waits (256 x 5120 x 5120 16.3 against 22.2).  4-bit
-    // a: the plain ring's steps are twice as long (64 x 5120 x 5120 8.7 us against 10.6 in steps of 128)
-    if constexpr (AF == MX_FP8) {
-        const int64_t tiles64 = ((a.M + 63) / 64) * ((a.N + 63) / 64);
-        if (tiles64 <= 256 && (((uintptr_t)a.As | (uintptr_t)a.Ws | (uintptr_t)a.ldas | (uintptr_t)a.ldws) & 3) == 0) {
-            auto* k = &k_mx_stream<EXACT, ODT>;
-            if (int rc = mx_room<MX_STREAM_LDS>((const void*)k)) return rc;
-            k<<<(unsigned)tiles64, 256, MX_STREAM_LDS, st>>>(a, (int)((a.M + 63) / 64));
-            return edadm_launch_status();
-        }
-    }
-    return launch_tile<AF, 2, 2, 1, 1, EXACT, ODT>(a, st);
 }
 
 // one object per type of a (they build in parallel); the entry point stands in the 8-bit one
