@@ -399,6 +399,33 @@ def test_product_long_rows(ops, mn, k, fmt):
         assert torch.equal(ops.mx_gemm(a, w, dtype=dtype), got)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n", [(5, 300), (100, 200), (1024, 2560), (4096, 4096)])
+@pytest.mark.parametrize("k", [100, 800, 1504, 2016, 2592])
+def test_product_scale_rows_off_dwords(ops, fmt, m, n, k):
+    """mx_quantize starts rows of scales at dwords; packed rows, which start anywhere, give the same bits"""
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    a = ops.mx_quantize(torch.randn(m, k, generator=g, device="cuda"), fmt)
+    w = ops.mx_quantize(torch.randn(n, k, generator=g, device="cuda") * 0.02, "mxfp4")
+    assert a.scales.stride(0) % 4 == 0 and a.scales.shape == (m, (k + 31) // 32)
+    pa, pw = ops.MXTensor(a.codes, a.scales.contiguous(), k, fmt), ops.MXTensor(w.codes, w.scales.contiguous(), k, "mxfp4")
+    assert pa.scales.stride(0) == (k + 31) // 32
+    for dtype in (torch.float32, torch.bfloat16):
+        got = ops.mx_gemm(a, w, dtype=dtype)
+        check_product(got, ops.mx_dequantize(a).double(), ops.mx_dequantize(w).double(), None, dtype, fmt)
+        assert torch.equal(ops.mx_gemm(pa, pw, dtype=dtype), got)
+
+
+def test_scale_rows_of_more_dimensions(ops):
+    """leading dimensions fold into rows whatever the scale pitch: no copy, the same values"""
+    x = torch.randn(3, 5, 7, 100, device="cuda")
+    q = ops.mx_quantize(x, "mxfp8")
+    assert q.scales.shape == (3, 5, 7, 4) and ops.mx_quantize(x[..., :90], "mxfp8").scales.shape == (3, 5, 7, 3)
+    q = ops.mx_quantize(x[..., :90], "mxfp8")
+    assert q._rows()[2].data_ptr() == q.scales.data_ptr()
+    same(ops.mx_dequantize(q), ops.mx_dequantize(ops.mx_quantize(x[..., :90].reshape(-1, 90), "mxfp8")).reshape(3, 5, 7, 90))
+
+
 @pytest.mark.parametrize("m", [1, 2, 3, 16, 17, 32, 33])
 @pytest.mark.parametrize("n", [64, 4100, 8200])
 @pytest.mark.parametrize("fmt", FMTS)
