@@ -6,7 +6,7 @@
 // elements of block q of row r; an 8-bit operand's lane holds elements 16 q .. 16 q + 15 of each half of row r; either way lane l gives
 // the scale of block q of row r.  w goes in as the first operand, so that a lane ends up with four neighbouring columns of one output row.
 //
-// What bounds it: one to 32 rows, reading w (k_mx_rows); few tiles, the way to memory; many, the matrix cores and the clock they leave
+// What bounds it: few rows or few columns, reading w (k_mx_rows); few tiles, the way to memory; many, the matrix cores and the clock they leave
 // (k_mx_tile): the instructions alone, operands in registers, reach 3.6 PFLOP/s with 8-bit a (1.72 GHz held) and 6.6
 // with 4-bit a (1.58 GHz); 8192 x 10240 x 5120 runs at 2.5 (8-bit), 8192 x 8192 x 8192 at 4.0 (4-bit).
 //
@@ -102,12 +102,12 @@ template <int ODT> __device__ __forceinline__ void mx_out4(const MxArgs& a, int6
     }
 }
 
-// ------------------------------------------------------------------------------------------------ few rows
+// ------------------------------------------------------------------------------------------------ few rows, or few of rows and columns
 // A workgroup owns 16 MT rows and 16 NT columns; its waves (as many as the launch gives it) take pairs of K-steps of 128 in turn, so
 // that every cache line of w (128 bytes = a pair of a row) is read by one wave, fetch their operands straight into registers, a pair
 // ahead of the one they multiply, and add their sums in LDS in the order of the waves.  Bound by reading w once: 1 x 5120 x 5120 6.9 us
-// in a graph (3.4 of them what any launch takes; 13.9 MB), 1 x 10240 x 10240 16.4 us, 4.3 TB/s behind the launch.  Every load is made
-// without a condition (a conditional 16-byte load was split into four).
+// in a graph (3.4 of them what any launch takes; 13.9 MB), 1 x 10240 x 10240 16.4 us, 4.3 TB/s behind the launch.  The end of K is
+// loaded without conditions (a conditional 16-byte load was split into four there).
 typedef uint32_t mx_u32 __attribute__((aligned(1)));                  // rows of scales start at any byte
 typedef uint32_t mx_u64 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t mx_u128 __attribute__((ext_vector_type(4), aligned(1)));
@@ -683,13 +683,16 @@ template <int AF, int WM, int WN, int MT, int NT, bool EXACT, int ODT> static in
 template <int AF, bool EXACT, int ODT> static int launch_mx(const MxArgs& a, hipStream_t st) {
     // the tiled kernel's 32-bit row offsets: 256 rows of a and of w under 4 GB
     const bool fits = a.lda < (1 << 23) && a.ldw < (1 << 23) && a.ldas < (1 << 23) && a.ldws < (1 << 23);
-    // few rows: 32 x 5120 x 5120 10.6 us there and 12.2 on 64 x 64 tiles, 48 x 5120 x 5120 13.6 and 12.4
-    if (a.M <= 32 || !fits) return launch_rows<AF, EXACT, ODT>(a, st);
+    // few rows, or few blocks of 32 x 32: K is split over the waves there, and a workgroup a CU reads its part at once where a tile walks
+    // K from end to end.  Weights from memory / in the caches, 8-bit a: 96 x 2560 x 2560 7.0 / 6.5 us there and 10.4 / 6.1 on 64 x 64
+    // tiles, 128 x 2560 x 2560 (320 blocks) 11.2 / 10.9 and 10.4 / 6.1; 64 x 1280 x 5120 11.3 / 10.1 and 18.2 / 9.4; 32 x 5120 x 5120
+    // 11.9 / 10.1 and 18.2 / 9.2, 48 x 5120 x 5120 14.9 / 13.4 and 18.3 / 9.3
+    if (a.M <= 32 || !fits || ((a.M + 31) / 32) * ((a.N + 31) / 32) <= 256) return launch_rows<AF, EXACT, ODT>(a, st);
     // The tile of least cost, in microseconds with 8-bit a and k = K / 1024 (4-bit a: two thirds of k): t tiles a CU of a full chip take
     // t (a + b k), and few tiles are no faster than c + d k min(t, r), r of them sharing a CU while they wait for memory.  Constants fitted
     // to 40 shapes (M 64 .. 32768, N 320 .. 10240, K 64 .. 10240), two sides of each choice: 8192 x 10240 x 5120 339 us on 256 x 256 and 369
     // on 256 x 192; 4096 x 5120 x 5120, 4-bit a, 81 and 69; 8192 x 8192 x 512 75 on 256 x 256, whose start and way out nothing hides, and 59
-    // on 128 x 128, two of which share a CU; 600 x 3000 x 8000 48 on 128 x 128 and 38 on 64 x 128; 128 x 5120 x 5120 15 on 64 x 128, 13 on
+    // on 128 x 128, two of which share a CU; 600 x 3000 x 8000 48 on 128 x 128 and 38 on 64 x 128; 128 x 5120 x 5120 12 on 64 x 128, 10.5 on
     // 64 x 64.
     static const struct { int bm, bn; float a, b, c, d; int r; } tiles[] = {{256, 256, 13.f, 11.f, 10.f, 8.5f, 1},
                                                                           {256, 192, 9.f, 8.7f, 8.f, 7.f, 1},

@@ -400,6 +400,22 @@ def test_product_long_rows(ops, mn, k, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("k", [31, 64, 160, 288, 544, 1000, 1056, 1280, 1504, 2592])
+@pytest.mark.parametrize("m,n", [(33, 4095), (96, 2560), (97, 2561), (511, 511), (513, 513), (1000, 257), (4097, 33), (8161, 31), (300, 1001)])
+def test_product_few_blocks(ops, m, n, k, fmt):
+    """both sides of 256 blocks of 32 x 32, where the product changes from waves that split K to 64 x 64 tiles, over every kind of K"""
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    a = ops.mx_quantize(torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(k, generator=g, device="cuda")), fmt)
+    w = ops.mx_quantize(torch.randn(n, k, generator=g, device="cuda") * 0.02, "mxfp4")
+    va, vw = ops.mx_dequantize(a).double(), ops.mx_dequantize(w).double()
+    bias = torch.randn(n, generator=g, device="cuda")
+    for dtype in DTYPES:
+        got = ops.mx_gemm(a, w, bias=bias, dtype=dtype)
+        check_product(got, va, vw, bias, dtype, fmt)
+        assert torch.equal(ops.mx_gemm(a, w, bias=bias, dtype=dtype), got)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,n", [(5, 300), (100, 200), (1024, 2560), (4096, 4096)])
 @pytest.mark.parametrize("k", [100, 800, 1504, 2016, 2592])
 def test_product_scale_rows_off_dwords(ops, fmt, m, n, k):
